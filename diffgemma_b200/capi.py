@@ -23,6 +23,7 @@ DG_ERR_ALIGNMENT = -7
 DG_DEV_WAIT_TIMEOUT = 1
 DG_DEV_SMEM_LAYOUT = 3
 DG_DEV_BAD_SHAPE = 2
+DG_DEV_NOT_FINITE = 4
 
 MASK_NONE, MASK_WINDOW_UNIFORM, MASK_WINDOW_PER_ROW, MASK_CAUSAL = 0, 1, 2, 3
 ROPE_SPLIT_HALF, ROPE_PROPORTIONAL = 0, 1
@@ -97,6 +98,16 @@ SIGNATURES = {
     "dg_host_pipe_destroy": (_i32, [_vp]),
     "dg_host_pipe_set_deferred_launch": (_i32, [_vp, _i32]),
     "dg_attn_denoise_bitmap": (_i32, [_vp, _pd, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "dg_kv8_create": (_i32, [_vp, _pd, _u64, C.POINTER(_vp)]),
+    "dg_kv8_destroy": (_i32, [_vp]),
+    "dg_kv8_capacity": (_u64, [_vp]),
+    "dg_kv8_append": (_i32, [_vp, _pd, _vp, _u64, _u64, _u64, _vp, _vp, _vp]),
+    "dg_kv8_load": (_i32, [_vp, _u64, _u64, _vp, _vp]),
+    "dg_kv8_read": (_i32, [_vp, _vp, _vp, _u64, _u64]),
+    "dg_kv8_denoise": (_i32, [_vp, _pd, C.POINTER(_vp), C.POINTER(_u32), C.POINTER(_u64), _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _vp]),
+    "dg_kv8_key_weights": (_i32, [_vp, _pd, _vp, _u32, _vp, _vp, _vp, _u64, C.c_float]),
+    "dg_kv8_evict": (_i32, [_vp, _vp, _u32, _vp, _u64, _u32, _u32, _vp, _vp, _vp, _u64]),
     "dg_attn_partial": (_i32, [_vp, _pd, _vp, _u32, _u32, _u32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "dg_attn_merge_local": (_i32, [_vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "dg_attn_merge_nccl": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32]),

@@ -1,0 +1,456 @@
+// Attention of canvas rows over caches held in 8 bits (csrc/dg_kv8.cuh has the format).
+//
+// One CTA: 128 GQA-stacked query rows of one KV head (row R -> canvas row R / G, head R % G), one range of key tiles, 256
+// value columns (a head_dim-512 layer takes two CTAs, both computing the scores).  One pass over the tiles with the running
+// maximum and sum of the softmax:
+//   S = (q1 + q2) K          2 x D / 32 MMAs (M 128, N 128, K 32), K as the cache holds it
+//   x = s * c 2^ek + ev - m  the block's scales are powers of two: that of K multiplies, that of V shifts the exponent
+//   P = 2^x = p1 + p2        e4m3 + e5m2 in tensor memory, over the columns that S occupied
+//   O += (p1 + p2) V         8 MMAs (M 128, N 256, K 32)
+//   l += 2^-ev sum P         in fp32, from P before it is rounded
+// m follows the largest x with a lag of at most 2^LAG (O is rescaled only beyond it), so P <= 2^8 stays inside e4m3.  p2 in
+// e5m2 reaches 2^-16, 2^-21 of the largest weight: a strong first token beside 10^5 weak ones loses none of them.
+// Tiles of the canvas come as two terms as well (K = k1 + k2, V = v1 + v2: the rows' bf16 values) and pass twice.
+//
+// Per 128 keys and 256 dims: 2,048 cycles of MMA, 64 KB from L2 / HBM, 256 KB of shared-memory traffic (Q 128, K 64 as
+// operands read twice, V 64 likewise ... half of what bf16 operands move), 16,384 exponentials (1,024 cycles).
+#include "dg_kv8.cuh"
+
+namespace dg {
+namespace kv8 {
+
+constexpr uint32_t T_S = 0, T_O = 256;          // tensor memory: two S buffers of 128 columns, O
+constexpr float LAG = 3.0f, LIFT = 5.0f;        // 2^(LAG + LIFT) = 256 <= 448
+enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V_FULL = 8, B_V_EMPTY = 10, B_S_FULL = 12, B_P_FULL = 14, B_PV = 16, N_BARS = 18 };
+
+template <uint32_t D> struct Cfg {
+  static constexpr uint32_t PARTS = D == 256 ? 4 : 2;           // softmax threads of a row
+  static constexpr uint32_t COLS = BLK / PARTS, OCOLS = 256 / PARTS;   // score and output columns of each
+  static constexpr uint32_t SM_WARPS = 4 * PARTS, W_K = SM_WARPS, W_V = W_K + 1, W_MMA = W_K + 2, THREADS = 32 * (SM_WARPS + 3);
+  static constexpr uint32_t KU = D / 256;                       // K units of a tile (32 KB each)
+  static constexpr uint32_t NK = 2, NV = D == 256 ? 2 : 1;   // stages
+  static constexpr uint32_t Q_BYTES = 2 * BLK * D;
+  static constexpr uint32_t O_K = Q_BYTES, O_V = O_K + NK * UNIT, O_X = O_V + NV * UNIT;
+  static constexpr uint32_t X_BYTES = 2 * PARTS * BLK * 4;      // row maxima of a row's threads, two parities
+  static constexpr uint32_t O_BAR = O_X + X_BYTES, SMEM = O_BAR + N_BARS * 8 + 16;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+};
+
+template <uint32_t N>
+__device__ __forceinline__ void bar_sync_quarter(uint32_t quarter) {   // the warps that share 32 rows
+  asm volatile("bar.sync %0, %1;" ::"r"(quarter + 1u), "n"(N) : "memory");
+}
+template <uint32_t PARTS>
+__device__ __forceinline__ float row_max(const float* x) {
+  float m = x[0];
+#pragma unroll
+  for (uint32_t i = 1; i < PARTS; ++i) m = fmaxf(m, x[i * BLK]);
+  return m;
+}
+
+template <uint32_t D>
+__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const __grid_constant__ AttnParams8 p) {
+  typedef Cfg<D> cf;
+  constexpr uint32_t PARTS = cf::PARTS, COLS = cf::COLS, GR = COLS / 32;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t s0 = smem_u32(smem);
+  volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + cf::O_BAR + N_BARS * 8);   // {abort, tmem}
+  volatile uint32_t* abort_flag = &ctl[0];
+  const uint32_t bars = s0 + cf::O_BAR;
+  auto bar = [&](uint32_t i) { return bars + i * 8u; };
+  float* xch = reinterpret_cast<float*>(smem + cf::O_X);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+
+  grid_launch_dependents();
+  if (s0 & 1023u) {   // the swizzled operands need the window itself aligned
+    if (tid == 0) dev_status_set(p.status, DG_DEV_SMEM_LAYOUT, KID_ATTN, blockIdx.x, s0);
+    return;
+  }
+  // which sequence, row tile, head, split and value half this CTA has
+  uint32_t b = 0;
+  for (uint32_t step = MAX_SEQ / 2; step > 0; step >>= 1)
+    if (b + step < p.n_seq && p.seq[b + step].first_cta <= blockIdx.x) b += step;
+  const Seq& sq = p.seq[b];
+  uint32_t item = blockIdx.x - sq.first_cta;
+  const uint32_t z = item % cf::KU;
+  item /= cf::KU;
+  const uint32_t mt = item % p.MT;
+  item /= p.MT;
+  const uint32_t kvh = item % p.Hkv, split = item / p.Hkv;
+  const MaskParams mk = seq_mask(p, sq.n_keys);
+  const uint32_t rows_per_head = p.C * p.G;
+  const uint32_t R_last = (mt + 1) * BLK < rows_per_head ? (mt + 1) * BLK - 1 : rows_per_head - 1;
+  const Tiles ts = tiles_of(mk, mt * BLK / p.G, R_last / p.G);
+  const uint32_t n0 = split_cut(ts, split, sq.n_splits), n1 = split_cut(ts, split + 1, sq.n_splits);
+  const uint32_t n_local = n1 - n0;
+
+  if (tid == 0) {
+    ctl[0] = 0u;
+    for (uint32_t i = 0; i < N_BARS; ++i)
+      mbar_init(bar(i), (i == B_P_FULL || i == B_P_FULL + 1) ? cf::SM_WARPS : 1u);
+    fence_mbar_init();
+  }
+  if (warp == cf::W_MMA) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(&ctl[1])), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl[1];
+  grid_wait();
+
+  const uint32_t head_tile = (b * p.Hkv + kvh) * p.n_ctiles;   // first canvas tile of this head
+  float m_used = -INFINITY, l_run = 0.f;
+  const uint32_t quarter = warp & 3u, part = warp >> 2;        // softmax warps: rows 32 quarter + lane, columns 32 part ..
+  const uint32_t r = quarter * 32u + lane;
+
+  if (warp < cf::SM_WARPS) {
+    const uint32_t R = mt * BLK + r;
+    const bool valid = R < rows_per_head;
+    const RowVis rv = mask_row(mk, valid ? R / p.G : 0u);
+    const float c_row = valid ? p.q_row[(size_t(b) * p.Hkv + kvh) * p.MT * BLK + R].x : 0.f;
+    const bool warp_on = mt * BLK + quarter * 32u < rows_per_head;   // any row of this warp
+    const uint32_t t_lane = tmem + ((quarter * 32u) << 16);
+    for (uint32_t n = 0; n < n_local; ++n) {
+      const uint32_t t = n0 + n, sb = n & 1u;
+      const bool cached = t < ts.nA;
+      const uint32_t blk = cached ? ts.a0 + t : t - ts.nA;
+      int ek, ev;
+      if (cached) {
+        ek = sq.k_exp[size_t(kvh) * sq.blocks + blk];
+        ev = sq.v_exp[size_t(kvh) * sq.blocks + blk];
+      } else {
+        ek = p.c_kexp[head_tile + blk];
+        ev = p.c_vexp[head_tile + blk];
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(B_S_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
+      if (!warp_on) {
+        // rows behind the last one: their P stays whatever it is, no row of the output reads it
+        if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+        continue;
+      }
+      tc_fence_after();
+      uint32_t s[GR][32];
+#pragma unroll
+      for (uint32_t g = 0; g < GR; ++g) tmem_ld32(t_lane + T_S + sb * 128u + part * COLS + g * 32u, s[g]);
+      tmem_wait_ld();
+      const uint32_t k0 = (cached ? blk * BLK : mk.kv_len + blk * BLK) + part * COLS;
+      const uint32_t lo = cached ? rv.lo : rv.can_lo, hi = cached ? mk.pre_hi : rv.can_hi;
+      if (k0 < lo || k0 + COLS > hi) {
+#pragma unroll
+        for (uint32_t g = 0; g < GR; ++g) {
+          const uint32_t seen = mask_run16(lo, hi, k0 + g * 32u) | (mask_run16(lo, hi, k0 + g * 32u + 16u) << 16);
+#pragma unroll
+          for (uint32_t e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1u)) s[g][e] = 0xff800000u;
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (uint32_t g = 0; g < GR; ++g)
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 2)
+          mx[(e >> 1) & 3u] = max3_f32(mx[(e >> 1) & 3u], __uint_as_float(s[g][e]), __uint_as_float(s[g][e + 1]));
+      const float mine = max3_f32(max3_f32(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
+      // after this barrier all threads of a row have their scores in registers: P may overwrite them
+      float* xc = xch + sb * PARTS * BLK;
+      xc[part * BLK + r] = mine;
+      bar_sync_quarter<32 * PARTS>(quarter);
+      const float top = row_max<PARTS>(xc + r);
+      const float c = c_row * pow2i(ek);
+      const float m_new = top * c + float(ev);
+      const bool need = n == 0 || m_new > m_used + LAG;
+      if (n != 0 && __any_sync(0xffffffffu, need)) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_PV + ((n - 1u) & 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
+        tc_fence_after();
+        const float alpha = need ? (m_used == -INFINITY ? 0.f : fast_exp2(m_used - m_new)) : 1.0f;
+#pragma unroll 1
+        for (uint32_t cc = 0; cc < cf::OCOLS / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32(t_lane + T_O + part * cf::OCOLS + cc * 32u, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (uint32_t e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(t_lane + T_O + part * cf::OCOLS + cc * 32u, o);
+        }
+        tmem_wait_st();
+        l_run *= alpha;
+      }
+      if (need) m_used = m_new;
+      const float shift = (m_used == -INFINITY ? 0.f : -m_used) + float(ev) + LIFT;
+      const uint64_t c2 = pack_f32x2(c, c), sh2 = pack_f32x2(shift, shift);
+      uint64_t ls[2] = {0ull, 0ull};
+#pragma unroll
+      for (uint32_t g = 0; g < GR; ++g) {
+        uint32_t p1[8], p2[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 4) {
+          uint16_t a[2], d[2];
+#pragma unroll
+          for (uint32_t j = 0; j < 2; ++j) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[g][e + 2 * j]), __uint_as_float(s[g][e + 2 * j + 1])), c2, sh2), x0, x1);
+            const float q0 = fast_exp2(x0), q1 = fast_exp2(x1);
+            ls[j] = add_f32x2(ls[j], pack_f32x2(q0, q1));
+            const uint32_t h = pack_f16x2(q0, q1);
+            a[j] = e4m3x2_from_f16x2(h);
+            d[j] = e5m2x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(a[j])));
+          }
+          p1[e >> 2] = uint32_t(a[0]) | (uint32_t(a[1]) << 16);
+          p2[e >> 2] = uint32_t(d[0]) | (uint32_t(d[1]) << 16);
+        }
+        tmem_st8(t_lane + T_S + sb * 128u + part * (COLS / 4) + g * 8u, p1);
+        tmem_st8(t_lane + T_S + sb * 128u + 32u + part * (COLS / 4) + g * 8u, p2);
+      }
+      {
+        float a, d;
+        unpack_f32x2(add_f32x2(ls[0], ls[1]), a, d);
+        l_run = fmaf(a + d, pow2i(-ev), l_run);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+    }
+  } else if (warp == cf::W_K) {
+    if (lane == 0 && n_local > 0) {
+      mbar_expect_tx(bar(B_Q), cf::Q_BYTES);
+      const uint8_t* q = p.q_codes + ((size_t(b) * p.Hkv + kvh) * p.MT + mt) * cf::Q_BYTES;
+      for (uint32_t o = 0; o < cf::Q_BYTES; o += UNIT) bulk_load(s0 + o, q + o, UNIT, bar(B_Q));
+      uint32_t u = 0;
+      bool ok = true;
+      for (uint32_t t = n0; ok && t < n1; ++t) {
+        const bool cached = t < ts.nA;
+        const uint8_t* src = cached ? sq.k + (size_t(kvh) * sq.blocks + ts.a0 + t) * BLK * D
+                                    : p.c_k + size_t(head_tile + t - ts.nA) * 2u * BLK * D;
+        const uint32_t units = cached ? cf::KU : 2 * cf::KU;
+        for (uint32_t i = 0; i < units; ++i, ++u) {
+          const uint32_t st = u % cf::NK;
+          if (u >= cf::NK && !mbar_wait(bar(B_K_EMPTY + st), (u / cf::NK - 1u) & 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(bar(B_K_FULL + st), UNIT);
+          bulk_load(s0 + cf::O_K + st * UNIT, src + size_t(i) * UNIT, UNIT, bar(B_K_FULL + st));
+        }
+      }
+    }
+  } else if (warp == cf::W_V) {
+    if (lane == 0) {
+      uint32_t u = 0;
+      bool ok = true;
+      for (uint32_t t = n0; ok && t < n1; ++t) {
+        const bool cached = t < ts.nA;
+        const uint8_t* src = (cached ? sq.v + (size_t(kvh) * sq.blocks + ts.a0 + t) * BLK * D
+                                     : p.c_v + size_t(head_tile + t - ts.nA) * 2u * BLK * D) + size_t(z) * UNIT;
+        for (uint32_t i = 0; i < (cached ? 1u : 2u); ++i, ++u) {
+          const uint32_t st = u % cf::NV;
+          if (u >= cf::NV && !mbar_wait(bar(B_V_EMPTY + st), (u / cf::NV - 1u) & 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(bar(B_V_FULL + st), UNIT);
+          bulk_load(s0 + cf::O_V + st * UNIT, src + size_t(i) * BLK * D, UNIT, bar(B_V_FULL + st));
+        }
+      }
+    }
+  } else if (n_local > 0) {
+    // the whole warp runs the loop, one elected lane issues
+    constexpr uint32_t IDESC_QK = idesc_f8(128, 128, 0, 0), IDESC_P1 = idesc_f8(128, 256, 0, 1), IDESC_P2 = idesc_f8(128, 256, 1, 1);
+    const uint64_t dq = umma_smem_desc(s0, 16, 1024), dk = umma_smem_desc(s0 + cf::O_K, 16, 1024);
+    const uint64_t dv = umma_smem_desc(s0 + cf::O_V, SLAB, 1024);   // MN-major: 128-column chunks SLAB apart, 8-token groups 1024
+    bool ok = __all_sync(0xffffffffu, mbar_wait(bar(B_Q), 0u, abort_flag));
+    uint32_t uk = 0, uv = 0;
+    auto issue_qk = [&](uint32_t n) -> bool {
+      const bool cached = n0 + n < ts.nA;
+      const uint32_t units = cached ? cf::KU : 2 * cf::KU;
+      const uint32_t d_tmem = tmem + T_S + (n & 1u) * 128u;
+      for (uint32_t i = 0; i < units; ++i, ++uk) {
+        const uint32_t st = uk % cf::NK;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_K_FULL + st), (uk / cf::NK) & 1u, abort_flag))) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t kb = dk + uint64_t(st * (UNIT >> 4));
+#pragma unroll 1
+          for (uint32_t term = 0; term < 2; ++term) {
+            const uint64_t qa = dq + uint64_t((term * BLK * D + (i % cf::KU) * UNIT) >> 4);
+#pragma unroll
+            for (uint32_t sl = 0; sl < 2; ++sl)
+#pragma unroll
+              for (uint32_t kk = 0; kk < 4; ++kk)
+                mma_ss(d_tmem, qa + sl * (SLAB >> 4) + kk * 2u, kb + sl * (SLAB >> 4) + kk * 2u, IDESC_QK, (i | term | sl | kk) != 0u);
+          }
+          umma_commit(bar(B_K_EMPTY + st));
+          if (i + 1 == units) umma_commit(bar(B_S_FULL + (n & 1u)));
+        }
+        __syncwarp();
+      }
+      return true;
+    };
+    ok = ok && issue_qk(0);
+    for (uint32_t n = 0; ok && n < n_local; ++n) {
+      if (n + 1 < n_local && !issue_qk(n + 1)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag))) break;
+      const uint32_t units = n0 + n < ts.nA ? 1u : 2u;
+      const uint32_t pt = tmem + T_S + (n & 1u) * 128u;
+      for (uint32_t i = 0; ok && i < units; ++i, ++uv) {
+        const uint32_t st = uv % cf::NV;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_V_FULL + st), (uv / cf::NV) & 1u, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vb = dv + uint64_t(st * (UNIT >> 4));
+#pragma unroll
+          for (uint32_t ks = 0; ks < 4; ++ks) {
+            mma_ts(tmem + T_O, pt + ks * 8u, vb + ks * (4096u >> 4), IDESC_P1, (n | i | ks) != 0u);
+            mma_ts(tmem + T_O, pt + 32u + ks * 8u, vb + ks * (4096u >> 4), IDESC_P2, 1u);
+          }
+          umma_commit(bar(B_V_EMPTY + st));
+          if (i + 1 == units) {
+            umma_commit(bar(B_PV + (n & 1u)));
+            if (n + 1 == n_local) umma_commit(bar(B_O));
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ output (softmax warps)
+  if (warp < cf::SM_WARPS) {
+    bool have = __all_sync(0xffffffffu, n_local > 0 && !*abort_flag);
+    if (have) {
+      have = __all_sync(0xffffffffu, mbar_wait(bar(B_O), 0u, abort_flag));
+      tc_fence_after();
+    }
+    // the row's sum is its threads' sums
+    bar_sync_quarter<32 * PARTS>(quarter);
+    xch[part * BLK + r] = l_run;
+    bar_sync_quarter<32 * PARTS>(quarter);
+    float l = xch[r];
+#pragma unroll
+    for (uint32_t i = 1; i < PARTS; ++i) l += xch[i * BLK + r];
+    const bool direct = sq.n_splits == 1;
+    const float mul = direct ? (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) : 1.0f;   // a sum that is NaN stays one
+    const uint32_t t_lane = tmem + ((quarter * 32u) << 16);
+    // 32 x 32 pieces through a padded tile of dead shared memory: every store instruction writes whole lines
+    float* tile = reinterpret_cast<float*>(smem) + warp * (32 * 36);
+    size_t row_k[8];
+    bool valid_k[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+      const uint32_t rk = quarter * 32u + k * 4u + (lane >> 3), Rk = mt * BLK + rk;
+      valid_k[k] = Rk < rows_per_head;
+      const uint32_t Rc = valid_k[k] ? Rk : 0u;
+      row_k[k] = direct ? ((size_t(b) * p.C + Rc / p.G) * p.Hq + kvh * p.G + Rc % p.G) * D + z * 256u
+                        : (size_t(blockIdx.x) * BLK + rk) * 256u;
+    }
+#pragma unroll 1
+    for (uint32_t cc = 0; cc < cf::OCOLS / 32; ++cc) {
+      const uint32_t col = part * cf::OCOLS + cc * 32u;
+      uint32_t o[32];
+      if (have) {
+        tmem_ld32(t_lane + T_O + col, o);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 32; ++e) o[e] = 0u;
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e)
+        *reinterpret_cast<float4*>(tile + lane * 36u + e * 4u) =
+            make_float4(__uint_as_float(o[e * 4]) * mul, __uint_as_float(o[e * 4 + 1]) * mul, __uint_as_float(o[e * 4 + 2]) * mul,
+                        __uint_as_float(o[e * 4 + 3]) * mul);
+      __syncwarp();
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(tile + (k * 4u + (lane >> 3)) * 36u + (lane & 7u) * 4u);
+        if (!valid_k[k]) continue;
+        const size_t at = row_k[k] + col + (lane & 7u) * 4u;
+        if (direct)
+          *reinterpret_cast<uint2*>(p.out + at) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+        else
+          *reinterpret_cast<float4*>(p.ws_o + at) = v;
+      }
+      __syncwarp();
+    }
+    const uint32_t R = mt * BLK + r;
+    if (part == 0 && R < rows_per_head) {
+      if (!direct)
+        p.ws_ml[size_t(blockIdx.x) * BLK + r] = make_float2(m_used, l);
+      else if (p.lse != nullptr && z == 0)
+        p.lse[(size_t(b) * p.C + R / p.G) * p.Hq + kvh * p.G + R % p.G] =
+            l == 0.f ? -INFINITY : (m_used - LIFT + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+
+  if (*abort_flag) {
+    if (tid == 0) dev_status_set(p.status, DG_DEV_WAIT_TIMEOUT, KID_ATTN, blockIdx.x, n_local);
+    if (warp == cf::W_K && lane == 0) {
+      const long long c0 = clock64();
+      while (clock64() - c0 < 2000000ll) {}   // ~1 ms: far longer than any load in flight
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == cf::W_MMA) tmem_dealloc(tmem, 512);
+}
+
+// Splits of a row joined: a warp per row and 256 columns, the splits in order.  A split without keys has m = -inf.
+__global__ void __launch_bounds__(256) dg_kv8_merge_kernel(const __grid_constant__ AttnParams8 p) {
+  grid_launch_dependents();
+  grid_wait();
+  const uint32_t lane = threadIdx.x & 31u, b = blockIdx.y, KU = p.D / 256u;
+  const Seq& sq = p.seq[b];
+  const uint32_t x = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (sq.n_splits == 1 || x >= p.C * p.Hq * KU) return;
+  const uint32_t z = x % KU, row = x / KU, i = row / p.Hq, h = row % p.Hq, kvh = h / p.G;
+  const uint32_t R = i * p.G + h % p.G, mt = R / BLK, r = R % BLK, S = sq.n_splits;
+  const uint32_t stride = p.Hkv * p.MT * KU, first = sq.first_cta + (kvh * p.MT + mt) * KU + z;
+  float m = -INFINITY;
+  for (uint32_t s = lane; s < S; s += 32u) m = fmaxf(m, p.ws_ml[size_t(first + s * stride) * BLK + r].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (uint32_t s = 0; s < S; ++s) {
+    const size_t at = size_t(first + s * stride) * BLK + r;
+    const float2 ml = p.ws_ml[at];
+    const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * 256u + lane * 8u);
+    const float4 a = src[0], c = src[1];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float w = fast_exp2(ml.x - m);
+    l = fmaf(w, ml.y, l);
+    acc[0] = fmaf(w, a.x, acc[0]); acc[1] = fmaf(w, a.y, acc[1]); acc[2] = fmaf(w, a.z, acc[2]); acc[3] = fmaf(w, a.w, acc[3]);
+    acc[4] = fmaf(w, c.x, acc[4]); acc[5] = fmaf(w, c.y, acc[5]); acc[6] = fmaf(w, c.z, acc[6]); acc[7] = fmaf(w, c.w, acc[7]);
+  }
+  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  const size_t orow = (size_t(b) * p.C + i) * p.Hq + h;
+  *reinterpret_cast<uint4*>(p.out + orow * p.D + z * 256u + lane * 8u) =
+      make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                 pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+  if (p.lse != nullptr && z == 0 && lane == 0) p.lse[orow] = l == 0.f ? -INFINITY : (m - LIFT + log2f(l)) * 0.6931471805599453f;
+}
+
+cudaError_t configure_attn() {
+  cudaError_t e = cudaFuncSetAttribute(dg_kv8_attn_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<256>::SMEM));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(dg_kv8_attn_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<512>::SMEM));
+  return e;
+}
+
+cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n_ctas);
+  cfg.blockDim = dim3(p.D == 256 ? Cfg<256>::THREADS : Cfg<512>::THREADS);
+  cfg.dynamicSmemBytes = p.D == 256 ? Cfg<256>::SMEM : Cfg<512>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = p.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<512>, p);
+  if (e != cudaSuccess || most_splits == 1) return e;
+  cfg.gridDim = dim3((p.C * p.Hq * (p.D / 256u) + 7u) / 8u, p.n_seq);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel, p);
+}
+
+}  // namespace kv8
+}  // namespace dg

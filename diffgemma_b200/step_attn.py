@@ -216,6 +216,72 @@ class KvCache:
             pass
 
 
+class KvCache8:
+    """dg_kv8: one layer's cache for one stream in 8 bits: e4m3 codes, a power-of-two scale for each 128 slots and KV head."""
+
+    def __init__(self, ctx: Context, layer: AttnLayer, capacity_tokens: int):
+        self.ctx = ctx
+        self.layer = layer
+        self.desc = layer.c_desc()
+        h = C.c_void_p()
+        check(ctx.lib.dg_kv8_create(ctx.h, C.byref(self.desc), capacity_tokens, C.byref(h)), "dg_kv8_create")
+        self.h = h
+        ctx._dependents.add(self)
+
+    @property
+    def capacity(self) -> int:
+        return int(self.ctx.lib.dg_kv8_capacity(self.h))
+
+    def _rows(self, k, v):
+        shape = (k.shape[0], self.layer.n_kv_heads, self.layer.head_dim)
+        assert k.dtype == v.dtype == torch.bfloat16 and tuple(k.shape) == tuple(v.shape) == shape, "bf16 [n, Hkv, D]"
+        return k.shape[0]
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, n_keys: int, pos: int | None = None, kw: torch.Tensor | None = None) -> None:
+        """Raw k, v [n, Hkv, D] into slots [n_keys, n_keys + n): norm, RoPE at positions pos.. (None: n_keys), 8 bits."""
+        n = self._rows(k, v)
+        check(self.ctx.lib.dg_kv8_append(self.ctx.h, C.byref(self.desc), self.h, n_keys, n_keys if pos is None else pos, n, _ptr(k),
+                                         _ptr(v), _ptr(kw)), "dg_kv8_append")
+
+    def load(self, k: torch.Tensor, v: torch.Tensor, n_keys: int = 0) -> None:
+        """Rows that are ready (K normed and rotated already) into slots [n_keys, n_keys + n)."""
+        n = self._rows(k, v)
+        if n:
+            check(self.ctx.lib.dg_kv8_load(self.h, n_keys, n, _ptr(k), _ptr(v)), "dg_kv8_load")
+
+    def read(self, slot0: int, n: int):
+        """Slots [slot0, slot0 + n) as bf16 k, v [n, Hkv, D]."""
+        lay = self.layer
+        k = torch.empty((n, lay.n_kv_heads, lay.head_dim), dtype=torch.bfloat16, device=f"cuda:{self.ctx.device}")
+        v = torch.empty_like(k)
+        if n:
+            check(self.ctx.lib.dg_kv8_read(self.h, _ptr(k), _ptr(v), slot0, n), "dg_kv8_read")
+        return k, v
+
+    def evict_to(self, to: "KvCache8", n_keys: int, weights: torch.Tensor, n_keep: int, n_recent: int = 0, kept=None, weights_out=None):
+        """The n_recent last tokens and the n_keep - n_recent of largest weight before them, into `to` (dg_kv8_evict).
+        weights: fp32 [Hkv, >= n_keys].  Returns the slots they had, int32 [Hkv, n_keep]."""
+        heads = self.layer.n_kv_heads
+        if kept is None:
+            kept = torch.empty((heads, n_keep), dtype=torch.int32, device=weights.device)
+        assert weights.dtype == torch.float32 and weights.shape[0] == heads and kept.shape == (heads, n_keep)
+        assert weights_out is None or (weights_out.dtype == torch.float32 and weights_out.shape[0] == heads)
+        check(self.ctx.lib.dg_kv8_evict(self.ctx.h, self.h, n_keys, _ptr(weights), weights.shape[1], n_keep, n_recent, to.h, _ptr(kept),
+                                        _ptr(weights_out), 0 if weights_out is None else weights_out.shape[1]), "dg_kv8_evict")
+        return kept
+
+    def close(self) -> None:
+        if self.h:
+            self.ctx.lib.dg_kv8_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class CanvasAttention:
     """The hot path for one layer: stage 1 (qk_rope_kv), stage 2 (attention), or both fused."""
 
@@ -260,6 +326,34 @@ class CanvasAttention:
         check(self.lib.dg_attn_denoise(self.ctx.h, C.byref(self.desc), kv_arr, len_arr, B, _ptr(q), _ptr(k), _ptr(v),
                                        _ptr(qw), _ptr(kw), _ptr(out)), "dg_attn_denoise")
         return out
+
+    def denoise_kv8(self, kvs, n_keys, q, k=None, v=None, qw=None, kw=None, out=None, pos=None, with_lse: bool = False,
+                    with_q_rot: bool = False):
+        """denoise() over caches held in 8 bits (dg_kv8_denoise).  q: [B,C,Hq,D], k, v: [B,C,Hkv,D] (None: the cached keys
+        alone); n_keys and pos: cached tokens and first position of each canvas (pos None: n_keys).  Returns out, or a tuple
+        with lse [B,C,Hq] and the rotated queries behind it where asked for."""
+        B, lay = len(kvs), self.layer
+        assert q.dtype == torch.bfloat16 and q.shape == (B, lay.canvas, lay.n_q_heads, lay.head_dim)
+        assert (k is None) == (v is None) and (k is None or k.shape == v.shape == (B, lay.canvas, lay.n_kv_heads, lay.head_dim))
+        out = torch.empty_like(q) if out is None else out
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
+        q_rot = torch.empty_like(q) if with_q_rot else None
+        check(self.lib.dg_kv8_denoise(self.ctx.h, C.byref(self.desc), (C.c_void_p * B)(*[kv.h for kv in kvs]), (C.c_uint32 * B)(*n_keys),
+                                      None if pos is None else (C.c_uint64 * B)(*pos), B, _ptr(q), _ptr(k), _ptr(v), _ptr(qw), _ptr(kw),
+                                      _ptr(out), _ptr(lse), _ptr(q_rot)), "dg_kv8_denoise")
+        if not (with_lse or with_q_rot):
+            return out
+        return tuple(t for t in (out, lse, q_rot) if t is not None)
+
+    def key_weights(self, kv: KvCache8, n_keys: int, q_rot, lse, weights, decay: float = 1.0):
+        """weights = decay * weights + what each cached key drew of the softmax of these rows (dg_kv8_key_weights).  q_rot
+        [C,Hq,D] and lse [C,Hq] as denoise_kv8 returned them; weights: fp32 [Hkv, >= n_keys], updated in place."""
+        lay = self.layer
+        assert q_rot.dtype == torch.bfloat16 and q_rot.shape[-3:] == (lay.canvas, lay.n_q_heads, lay.head_dim)
+        assert lse.dtype == weights.dtype == torch.float32 and weights.shape[0] == lay.n_kv_heads
+        check(self.lib.dg_kv8_key_weights(self.ctx.h, C.byref(self.desc), kv.h, n_keys, _ptr(q_rot), _ptr(lse), _ptr(weights),
+                                          weights.shape[1], decay), "dg_kv8_key_weights")
+        return weights
 
     def denoise_host(self, kvs, kv_lens, q, k, v, out, qw=None, kw=None):
         """Same with HOST tensors q, k, v, out (pinned recommended); synchronous."""

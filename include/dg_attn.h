@@ -41,6 +41,7 @@ enum {
   DG_ERR_ALIGNMENT = -7,     /* a device pointer is not 16-byte aligned                         */
   DG_DEV_WAIT_TIMEOUT = 1,   /* a bounded device-side wait gave up (kernel unwound cleanly)     */
   DG_DEV_BAD_SHAPE = 2,      /* device-side shape assertion                                     */
+  DG_DEV_NOT_FINITE = 4,     /* a number that was to be held in 8 bits is not finite: it is held as zero */
   DG_DEV_SMEM_LAYOUT = 3     /* a kernel's shared-memory map did not fit its (unaligned) window; it
                               * returned without doing anything                                  */
 };
@@ -314,6 +315,55 @@ typedef struct dg_topk_cfg {
 int32_t dg_attn_denoise_topk(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv* kv, uint32_t kv_len, const void* q,
                              const void* k, const void* v, const void* qw, const void* kw, const dg_topk_cfg* cfg,
                              void* out);
+
+/* ---- caches held in 8 bits -------------------------------------------------------------------
+ * A frozen prefix at half the memory of bf16, and what keeps it in bounds: attention over it, the weight that each of its
+ * keys draws, eviction by that weight.  No counterpart in the reference.
+ *
+ * K and V of each KV head are e4m3 codes with one power-of-two scale for each block of 128 slots:
+ *   value = code * 2^e,  e = the smallest integer in [-60, 60] with (largest magnitude of the block) <= 448 * 2^e,
+ * codes rounded to nearest even.  A value carries four significant bits down to 2^-14 of its block's largest and an absolute
+ * error of 2^-19 of that below it.  What is not finite cannot be held: it is stored as zero and DG_DEV_NOT_FINITE is
+ * reported.  head_dim 256 or 512, rotary_dim a multiple of 16; linear caches.
+ *
+ * Tokens sit in slots [0, n_keys); the caller keeps n_keys.  RoPE positions are given apart from slots, because after an
+ * eviction they differ: `pos` is the position of the first new token.  Angles are computed in 64 bits (dg_kv_append's are
+ * 32-bit: up to 0.008 apart at position 131,072).  All pointers are device pointers unless said otherwise.              */
+typedef struct dg_kv8 dg_kv8;
+int32_t dg_kv8_create(dg_ctx* ctx, const dg_layer_desc* desc, uint64_t capacity_tokens, dg_kv8** out);
+int32_t dg_kv8_destroy(dg_kv8* kv);
+uint64_t dg_kv8_capacity(const dg_kv8* kv);      /* capacity_tokens rounded up to whole blocks */
+/* Raw keys and values (k, v: bf16 [n][Hkv][D]) into slots [n_keys, n_keys + n): K normed (weight kw, or NULL) and rotated to
+ * positions pos.., V normed where the layer does, both rounded to bf16 as the other cache stores them, then coded.  A block
+ * that holds tokens already is coded again as a whole, from the values it holds, at the scale that old and new need.     */
+int32_t dg_kv8_append(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* kv, uint64_t n_keys, uint64_t pos, uint64_t n,
+                      const void* k, const void* v, const void* kw);
+/* The same for rows that are ready (K normed and rotated already), on the stream of the cache's context.                */
+int32_t dg_kv8_load(dg_kv8* kv, uint64_t n_keys, uint64_t n, const void* k, const void* v);
+/* Slots [slot0, slot0 + n) as bf16 [n][Hkv][D] (exact), ordered on the context's stream; does not synchronise.          */
+int32_t dg_kv8_read(dg_kv8* kv, void* k_out, void* v_out, uint64_t slot0, uint64_t n);
+/* dg_attn_denoise over such caches: `batch` canvases of desc->canvas rows (1 for single tokens), each over slots
+ * [0, n_keys[b]) of kv[b] and, where k and v are given, over its own K and V, which enter as bf16 rows and are not stored
+ * (dg_kv8_append stores them once they are final).  k = v = NULL: the cached keys alone; a row that then sees none gives
+ * zeros.  pos[b] (host array; NULL: n_keys) is the position of canvas row 0.  A window counts positions and needs
+ * pos[b] = n_keys[b].  The same cache may serve several canvases.  out: bf16 [batch][C][Hq][D]; lse (or NULL): fp32
+ * [batch][C][Hq], ln of the sum of e^score over what a row sees, -inf where it sees nothing; q_rot (or NULL): the normed
+ * and rotated queries, bf16 [batch][C][Hq][D].                                                                          */
+int32_t dg_kv8_denoise(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* const* kv, const uint32_t* n_keys, const uint64_t* pos,
+                       uint32_t batch, const void* q, const void* k, const void* v, const void* qw, const void* kw, void* out,
+                       float* lse, void* q_rot);
+/* What each cached key drew of the softmax of one canvas's rows, added up over rows and the query heads of its KV head:
+ *   weights[h * ld + t] = decay * weights[h * ld + t] + sum e^(score - lse),   t < n_keys
+ * q_rot and lse as dg_kv8_denoise returned them for this canvas and cache; the mask is desc's (positions = slots).  decay 0:
+ * weights is written without being read; 1: plain sums.                                                                 */
+int32_t dg_kv8_key_weights(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* kv, uint32_t n_keys, const void* q_rot, const float* lse,
+                           float* weights, uint64_t ld, float decay);
+/* Keeps n_keep of n_keys tokens of each KV head in `to`, in order: the last n_recent, and of those before them the
+ * n_keep - n_recent with the largest weights (equal weights: the lower slot; NaN below every number).  kept: int32
+ * [Hkv][n_keep], the slots they had; weights_out (or NULL, row stride ld_out): their weights.  `to` is another cache of the
+ * same geometry and is overwritten from slot 0; heads keep different tokens, so windows no longer apply.               */
+int32_t dg_kv8_evict(dg_ctx* ctx, dg_kv8* from, uint32_t n_keys, const float* weights, uint64_t ld, uint32_t n_keep,
+                     uint32_t n_recent, dg_kv8* to, int32_t* kept, float* weights_out, uint64_t ld_out);
 
 /* ---- split-KV building blocks (multi-GPU, and the block-continuation state of the reference:
  * AttnBlockRange / attn_state, src/shaders/include/attention_device.metal:154-165) ------------ */
