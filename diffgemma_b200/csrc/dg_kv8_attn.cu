@@ -21,37 +21,60 @@ namespace kv8 {
 
 constexpr uint32_t T_S = 0, T_O = 256;          // tensor memory: two S buffers of 128 columns, O
 constexpr float LAG = 3.0f, LIFT = 5.0f;        // 2^(LAG + LIFT) = 256 <= 448
-enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V_FULL = 8, B_V_EMPTY = 10, B_S_FULL = 12, B_P_FULL = 14, B_PV = 16, N_BARS = 18 };
+constexpr uint32_t SM_WARPS = 16, GROUP_WARPS = 8, W_K = 16, W_V = 17, W_MMA = 18, THREADS = 19 * 32;
+// B_P_FULL of a tile counts its eight softmax warps and the bytes of its first V unit; B_V2_FULL those of a canvas tile's second
+enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V2_FULL = 8, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 13, B_REF = 15, N_BARS = 17 };
 
 template <uint32_t D> struct Cfg {
-  static constexpr uint32_t PARTS = D == 256 ? 4 : 2;           // softmax threads of a row
-  static constexpr uint32_t COLS = BLK / PARTS, OCOLS = 256 / PARTS;   // score and output columns of each
-  static constexpr uint32_t SM_WARPS = 4 * PARTS, W_K = SM_WARPS, W_V = W_K + 1, W_MMA = W_K + 2, THREADS = 32 * (SM_WARPS + 3);
   static constexpr uint32_t KU = D / 256;                       // K units of a tile (32 KB each)
-  static constexpr uint32_t NK = 2, NV = D == 256 ? 2 : 1;   // stages
+  static constexpr uint32_t NK = D == 256 ? 3 : 2, NV = D == 256 ? 2 : 1;   // stages
   static constexpr uint32_t Q_BYTES = 2 * BLK * D;
   static constexpr uint32_t O_K = Q_BYTES, O_V = O_K + NK * UNIT, O_X = O_V + NV * UNIT;
-  static constexpr uint32_t X_BYTES = 2 * PARTS * BLK * 4;      // row maxima of a row's threads, two parities
+  static constexpr uint32_t X_BYTES = (2 * 2 + 1) * BLK * 4;    // each group's row maxima (two threads a row); the reference
   static constexpr uint32_t O_BAR = O_X + X_BYTES, SMEM = O_BAR + N_BARS * 8 + 16;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
 
-template <uint32_t N>
-__device__ __forceinline__ void bar_sync_quarter(uint32_t quarter) {   // the warps that share 32 rows
-  asm volatile("bar.sync %0, %1;" ::"r"(quarter + 1u), "n"(N) : "memory");
+__device__ __forceinline__ void bar_sync_id(uint32_t id, uint32_t threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-template <uint32_t PARTS>
-__device__ __forceinline__ float row_max(const float* x) {
-  float m = x[0];
+// 32 weights of a row from their scores: two words of e4m3 codes and two of e5m2 codes for every eight; sums into ls
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t c2, uint64_t sh2, uint64_t (&ls)[2], uint32_t (&p1)[8], uint32_t (&p2)[8]) {
 #pragma unroll
-  for (uint32_t i = 1; i < PARTS; ++i) m = fmaxf(m, x[i * BLK]);
-  return m;
+  for (uint32_t e = 0; e < 32; e += 4) {
+    uint16_t a[2], d[2];
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      float x0, x1;
+      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), c2, sh2), x0, x1);
+      const float q0 = fast_exp2(x0), q1 = fast_exp2(x1);
+      ls[j] = add_f32x2(ls[j], pack_f32x2(q0, q1));
+      const uint32_t h = pack_f16x2(q0, q1);
+      a[j] = e4m3x2_from_f16x2(h);
+      d[j] = e5m2x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(a[j])));
+    }
+    p1[e >> 2] = uint32_t(a[0]) | (uint32_t(a[1]) << 16);
+    p2[e >> 2] = uint32_t(d[0]) | (uint32_t(d[1]) << 16);
+  }
+}
+__device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (uint32_t e = 0; e < 32; e += 2) mx[(e >> 1) & 3u] = max3_f32(mx[(e >> 1) & 3u], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+  return max3_f32(max3_f32(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
+}
+// scores of keys [k0, k0 + 32) that the row does not see become -inf
+__device__ __forceinline__ void hide32(uint32_t (&s)[32], uint32_t lo, uint32_t hi, uint32_t k0) {
+  if (k0 >= lo && k0 + 32u <= hi) return;
+  const uint32_t seen = mask_run16(lo, hi, k0) | (mask_run16(lo, hi, k0 + 16u) << 16);
+#pragma unroll
+  for (uint32_t e = 0; e < 32; ++e)
+    if (!((seen >> e) & 1u)) s[e] = 0xff800000u;
 }
 
 template <uint32_t D>
-__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const __grid_constant__ AttnParams8 p) {
+__global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_constant__ AttnParams8 p) {
   typedef Cfg<D> cf;
-  constexpr uint32_t PARTS = cf::PARTS, COLS = cf::COLS, GR = COLS / 32;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s0 = smem_u32(smem);
   volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + cf::O_BAR + N_BARS * 8);   // {abort, tmem}
@@ -83,14 +106,24 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
   const Tiles ts = tiles_of(mk, mt * BLK / p.G, R_last / p.G);
   const uint32_t n0 = split_cut(ts, split, sq.n_splits), n1 = split_cut(ts, split + 1, sq.n_splits);
   const uint32_t n_local = n1 - n0;
+  const uint32_t n_cached = ts.nA > n0 ? (ts.nA - n0 < n_local ? ts.nA - n0 : n_local) : 0u;   // cached tiles come first
+  // Units are numbered through the CTA's tiles, one of a cached tile, two of a canvas tile; unit u goes through stage u % stages.
+  // Waits until the last unit of tile n has been used, for a warp that has seen the one of tile n - 2 (K) or n - 2 (V) used: a
+  // canvas tile's first unit is waited for as well, so that no phase is skipped and its parity mistaken.
+  auto wait_unit = [&](uint32_t barrier, uint32_t stages, uint32_t n) -> bool {
+    const uint32_t u = n < n_cached ? n : 2u * n + 1u - n_cached;
+    bool ok = true;
+    if (n >= n_cached) ok = mbar_wait(bar(barrier + (u - 1u) % stages), ((u - 1u) / stages) & 1u, abort_flag);
+    return __all_sync(0xffffffffu, ok && mbar_wait(bar(barrier + u % stages), (u / stages) & 1u, abort_flag));
+  };
 
   if (tid == 0) {
     ctl[0] = 0u;
     for (uint32_t i = 0; i < N_BARS; ++i)
-      mbar_init(bar(i), (i == B_P_FULL || i == B_P_FULL + 1) ? cf::SM_WARPS : 1u);
+      mbar_init(bar(i), i >= B_REF ? GROUP_WARPS : i >= B_P_FULL ? GROUP_WARPS + 1u : 1u);
     fence_mbar_init();
   }
-  if (warp == cf::W_MMA) {
+  if (warp == W_MMA) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(&ctl[1])), 512);
     tmem_relinquish();
   }
@@ -102,18 +135,23 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
 
   const uint32_t head_tile = (b * p.Hkv + kvh) * p.n_ctiles;   // first canvas tile of this head
   float m_used = -INFINITY, l_run = 0.f;
-  const uint32_t quarter = warp & 3u, part = warp >> 2;        // softmax warps: rows 32 quarter + lane, columns 32 part ..
-  const uint32_t r = quarter * 32u + lane;
+  // Softmax: two groups of eight warps take alternate tiles, so that one's latencies lie under the other's work; two threads
+  // a row, 64 score columns each.
+  const uint32_t quarter = warp & 3u, grp = (warp >> 3) & 1u, part = (warp >> 2) & 1u;
+  const uint32_t r = quarter * 32u + lane;                     // row
+  float* ref = xch + 4 * BLK;                                  // what the exponents of the last decided tile refer to
 
-  if (warp < cf::SM_WARPS) {
+  if (warp < SM_WARPS) {
     const uint32_t R = mt * BLK + r;
     const bool valid = R < rows_per_head;
     const RowVis rv = mask_row(mk, valid ? R / p.G : 0u);
     const float c_row = valid ? p.q_row[(size_t(b) * p.Hkv + kvh) * p.MT * BLK + R].x : 0.f;
     const bool warp_on = mt * BLK + quarter * 32u < rows_per_head;   // any row of this warp
-    const uint32_t t_lane = tmem + ((quarter * 32u) << 16);
-    for (uint32_t n = 0; n < n_local; ++n) {
-      const uint32_t t = n0 + n, sb = n & 1u;
+    const uint32_t t_s = tmem + ((quarter * 32u) << 16) + T_S + grp * 128u + part * 64u;
+    const uint32_t t_o = tmem + ((quarter * 32u) << 16) + T_O + part * 128u;
+    float* xm = xch + grp * 2u * BLK + r;
+    for (uint32_t n = grp; n < n_local; n += 2) {
+      const uint32_t t = n0 + n, ph = (n >> 1) & 1u;
       const bool cached = t < ts.nA;
       const uint32_t blk = cached ? ts.a0 + t : t - ts.nA;
       int ek, ev;
@@ -124,85 +162,78 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
         ek = p.c_kexp[head_tile + blk];
         ev = p.c_vexp[head_tile + blk];
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(B_S_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
+      // head_dim 256: the scores are there when the tile's last K unit has been used
+      if (D == 256 ? !wait_unit(B_K_EMPTY, cf::NK, n) : !__all_sync(0xffffffffu, mbar_wait(bar(B_S_FULL + grp), ph, abort_flag))) break;
       if (!warp_on) {
         // rows behind the last one: their P stays whatever it is, no row of the output reads it
-        if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+        if (lane == 0) {
+          mbar_arrive(bar(B_REF + grp));
+          mbar_arrive(bar(B_P_FULL + grp));
+        }
         continue;
       }
       tc_fence_after();
-      uint32_t s[GR][32];
-#pragma unroll
-      for (uint32_t g = 0; g < GR; ++g) tmem_ld32(t_lane + T_S + sb * 128u + part * COLS + g * 32u, s[g]);
-      tmem_wait_ld();
-      const uint32_t k0 = (cached ? blk * BLK : mk.kv_len + blk * BLK) + part * COLS;
+      const uint32_t k0 = (cached ? blk * BLK : mk.kv_len + blk * BLK) + part * 64u;
       const uint32_t lo = cached ? rv.lo : rv.can_lo, hi = cached ? mk.pre_hi : rv.can_hi;
-      if (k0 < lo || k0 + COLS > hi) {
-#pragma unroll
-        for (uint32_t g = 0; g < GR; ++g) {
-          const uint32_t seen = mask_run16(lo, hi, k0 + g * 32u) | (mask_run16(lo, hi, k0 + g * 32u + 16u) << 16);
-#pragma unroll
-          for (uint32_t e = 0; e < 32; ++e)
-            if (!((seen >> e) & 1u)) s[g][e] = 0xff800000u;
-        }
+      uint32_t s[32];
+      tmem_ld32(t_s, s);
+      tmem_wait_ld();
+      hide32(s, lo, hi, k0);
+      float top = max32(s);
+      tmem_ld32(t_s + 32u, s);
+      tmem_wait_ld();
+      hide32(s, lo, hi, k0 + 32u);
+      top = fmaxf(top, max32(s));
+      xm[part * BLK] = top;
+      // the reference that the tile before was given
+      if (n != 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_REF + (grp ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (uint32_t g = 0; g < GR; ++g)
-#pragma unroll
-        for (uint32_t e = 0; e < 32; e += 2)
-          mx[(e >> 1) & 3u] = max3_f32(mx[(e >> 1) & 3u], __uint_as_float(s[g][e]), __uint_as_float(s[g][e + 1]));
-      const float mine = max3_f32(max3_f32(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
-      // after this barrier all threads of a row have their scores in registers: P may overwrite them
-      float* xc = xch + sb * PARTS * BLK;
-      xc[part * BLK + r] = mine;
-      bar_sync_quarter<32 * PARTS>(quarter);
-      const float top = row_max<PARTS>(xc + r);
+      const float m_prev = n != 0 ? ref[r] : -INFINITY;
+      bar_sync_id(1u + grp * 4u + quarter, 64u);
+      top = fmaxf(top, xm[(part ^ 1u) * BLK]);
       const float c = c_row * pow2i(ek);
       const float m_new = top * c + float(ev);
-      const bool need = n == 0 || m_new > m_used + LAG;
+      const bool need = n == 0 || m_new > m_prev + LAG;
+      const float m_ref = need ? m_new : m_prev;
+      if (part == 0) ref[r] = m_ref;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_REF + grp));
       if (n != 0 && __any_sync(0xffffffffu, need)) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_PV + ((n - 1u) & 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
+        // the outputs of the tile before: its last V unit has been used
+        if (!wait_unit(B_V_EMPTY, cf::NV, n - 1u)) break;
         tc_fence_after();
-        const float alpha = need ? (m_used == -INFINITY ? 0.f : fast_exp2(m_used - m_new)) : 1.0f;
+        const float alpha = need ? (m_prev == -INFINITY ? 0.f : fast_exp2(m_prev - m_new)) : 1.0f;
 #pragma unroll 1
-        for (uint32_t cc = 0; cc < cf::OCOLS / 32; ++cc) {
+        for (uint32_t cc = 0; cc < 4; ++cc) {
           uint32_t o[32];
-          tmem_ld32(t_lane + T_O + part * cf::OCOLS + cc * 32u, o);
+          tmem_ld32(t_o + cc * 32u, o);
           tmem_wait_ld();
 #pragma unroll
           for (uint32_t e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(t_lane + T_O + part * cf::OCOLS + cc * 32u, o);
+          tmem_st32(t_o + cc * 32u, o);
         }
-        tmem_wait_st();
-        l_run *= alpha;
       }
-      if (need) m_used = m_new;
-      const float shift = (m_used == -INFINITY ? 0.f : -m_used) + float(ev) + LIFT;
+      // this thread's sum may stand at an older reference
+      if (m_ref != m_used) {
+        l_run = m_used == -INFINITY ? 0.f : l_run * fast_exp2(m_used - m_ref);
+        m_used = m_ref;
+      }
+      const float shift = (m_ref == -INFINITY ? 0.f : -m_ref) + float(ev) + LIFT;
       const uint64_t c2 = pack_f32x2(c, c), sh2 = pack_f32x2(shift, shift);
       uint64_t ls[2] = {0ull, 0ull};
-#pragma unroll
-      for (uint32_t g = 0; g < GR; ++g) {
-        uint32_t p1[8], p2[8];
-#pragma unroll
-        for (uint32_t e = 0; e < 32; e += 4) {
-          uint16_t a[2], d[2];
-#pragma unroll
-          for (uint32_t j = 0; j < 2; ++j) {
-            float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[g][e + 2 * j]), __uint_as_float(s[g][e + 2 * j + 1])), c2, sh2), x0, x1);
-            const float q0 = fast_exp2(x0), q1 = fast_exp2(x1);
-            ls[j] = add_f32x2(ls[j], pack_f32x2(q0, q1));
-            const uint32_t h = pack_f16x2(q0, q1);
-            a[j] = e4m3x2_from_f16x2(h);
-            d[j] = e5m2x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(a[j])));
-          }
-          p1[e >> 2] = uint32_t(a[0]) | (uint32_t(a[1]) << 16);
-          p2[e >> 2] = uint32_t(d[0]) | (uint32_t(d[1]) << 16);
-        }
-        tmem_st8(t_lane + T_S + sb * 128u + part * (COLS / 4) + g * 8u, p1);
-        tmem_st8(t_lane + T_S + sb * 128u + 32u + part * (COLS / 4) + g * 8u, p2);
-      }
+      // P goes over the second half of the thread's own score columns, which it has in registers: 8 columns each of p1 of
+      // the first and second 32 keys, then p2
+      uint32_t p1[8], p2[8];
+      weights32(s, c2, sh2, ls, p1, p2);
+      tmem_st8(t_s + 40u, p1);
+      tmem_st8(t_s + 56u, p2);
+      tmem_ld32(t_s, s);
+      tmem_wait_ld();
+      hide32(s, lo, hi, k0);
+      weights32(s, c2, sh2, ls, p1, p2);
+      tmem_st8(t_s + 32u, p1);
+      tmem_st8(t_s + 48u, p2);
       {
         float a, d;
         unpack_f32x2(add_f32x2(ls[0], ls[1]), a, d);
@@ -211,9 +242,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+      if (lane == 0) mbar_arrive(bar(B_P_FULL + grp));
     }
-  } else if (warp == cf::W_K) {
+  } else if (warp == W_K) {
     if (lane == 0 && n_local > 0) {
       mbar_expect_tx(bar(B_Q), cf::Q_BYTES);
       const uint8_t* q = p.q_codes + ((size_t(b) * p.Hkv + kvh) * p.MT + mt) * cf::Q_BYTES;
@@ -233,7 +264,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
         }
       }
     }
-  } else if (warp == cf::W_V) {
+  } else if (warp == W_V) {
     if (lane == 0) {
       uint32_t u = 0;
       bool ok = true;
@@ -244,39 +275,41 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
         for (uint32_t i = 0; i < (cached ? 1u : 2u); ++i, ++u) {
           const uint32_t st = u % cf::NV;
           if (u >= cf::NV && !mbar_wait(bar(B_V_EMPTY + st), (u / cf::NV - 1u) & 1u, abort_flag)) { ok = false; break; }
-          mbar_expect_tx(bar(B_V_FULL + st), UNIT);
-          bulk_load(s0 + cf::O_V + st * UNIT, src + size_t(i) * BLK * D, UNIT, bar(B_V_FULL + st));
+          const uint32_t full = bar(i == 0 ? B_P_FULL + ((t - n0) & 1u) : B_V2_FULL);
+          mbar_expect_tx(full, UNIT);
+          bulk_load(s0 + cf::O_V + st * UNIT, src + size_t(i) * BLK * D, UNIT, full);
         }
       }
     }
   } else if (n_local > 0) {
-    // the whole warp runs the loop, one elected lane issues
-    constexpr uint32_t IDESC_QK = idesc_f8(128, 128, 0, 0), IDESC_P1 = idesc_f8(128, 256, 0, 1), IDESC_P2 = idesc_f8(128, 256, 1, 1);
-    const uint64_t dq = umma_smem_desc(s0, 16, 1024), dk = umma_smem_desc(s0 + cf::O_K, 16, 1024);
-    const uint64_t dv = umma_smem_desc(s0 + cf::O_V, SLAB, 1024);   // MN-major: 128-column chunks SLAB apart, 8-token groups 1024
+    // The whole warp runs the loop, one elected lane issues.  A wait costs this warp some 150 cycles in which it issues nothing;
+    // one before each group of 1,024 cycles of MMAs and one commit behind it keep the tensor pipe full (2,054 cycles for the 24
+    // MMAs of a 256-wide tile; two waits and two commits: 2,360), so V's bytes are counted where P's arrivals are and a K
+    // unit's release is the signal that scores are there.  Descriptors advance by adds on their low word (every operand lives
+    // below 256 KB: the address field cannot carry).
+    constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);           // 8-row groups 1024 apart, version 1, 128-byte swizzle
+    auto desc = [](uint32_t lo) { return (uint64_t(HI) << 32) | uint64_t(lo); };
+    constexpr uint32_t IDESC = idesc_f8(128, 128, 0, 0), IDESC_P1 = idesc_f8(128, 256, 0, 1), IDESC_P2 = idesc_f8(128, 256, 1, 1);
+    const uint32_t dq = ((s0 >> 4) & 0x3fffu) | (1u << 16), dk = (((s0 + cf::O_K) >> 4) & 0x3fffu) | (1u << 16);
+    const uint32_t dv = (((s0 + cf::O_V) >> 4) & 0x3fffu) | ((SLAB >> 4) << 16);   // MN-major: 128-column chunks SLAB apart
     bool ok = __all_sync(0xffffffffu, mbar_wait(bar(B_Q), 0u, abort_flag));
     uint32_t uk = 0, uv = 0;
     auto issue_qk = [&](uint32_t n) -> bool {
-      const bool cached = n0 + n < ts.nA;
-      const uint32_t units = cached ? cf::KU : 2 * cf::KU;
+      const uint32_t units = n < n_cached ? cf::KU : 2 * cf::KU;
       const uint32_t d_tmem = tmem + T_S + (n & 1u) * 128u;
       for (uint32_t i = 0; i < units; ++i, ++uk) {
         const uint32_t st = uk % cf::NK;
         if (!__all_sync(0xffffffffu, mbar_wait(bar(B_K_FULL + st), (uk / cf::NK) & 1u, abort_flag))) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t kb = dk + uint64_t(st * (UNIT >> 4));
-#pragma unroll 1
-          for (uint32_t term = 0; term < 2; ++term) {
-            const uint64_t qa = dq + uint64_t((term * BLK * D + (i % cf::KU) * UNIT) >> 4);
+          const uint32_t qa = dq + (((i % cf::KU) * UNIT) >> 4), kb = dk + st * (UNIT >> 4);
 #pragma unroll
-            for (uint32_t sl = 0; sl < 2; ++sl)
-#pragma unroll
-              for (uint32_t kk = 0; kk < 4; ++kk)
-                mma_ss(d_tmem, qa + sl * (SLAB >> 4) + kk * 2u, kb + sl * (SLAB >> 4) + kk * 2u, IDESC_QK, (i | term | sl | kk) != 0u);
+          for (uint32_t j = 0; j < 16; ++j) {   // term, slab, 32 dims
+            const uint32_t o = ((j >> 2) & 1u) * (SLAB >> 4) + (j & 3u) * 2u;
+            mma_ss(d_tmem, desc(qa + (j >> 3) * ((BLK * D) >> 4) + o), desc(kb + o), IDESC, j == 0 ? i != 0u : 1u);
           }
           umma_commit(bar(B_K_EMPTY + st));
-          if (i + 1 == units) umma_commit(bar(B_S_FULL + (n & 1u)));
+          if (D != 256 && i + 1 == units) umma_commit(bar(B_S_FULL + (n & 1u)));
         }
         __syncwarp();
       }
@@ -284,27 +317,28 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
     };
     ok = ok && issue_qk(0);
     for (uint32_t n = 0; ok && n < n_local; ++n) {
+      // (S of tile n + 1 goes where P of tile n - 1 was read by MMAs issued before)
       if (n + 1 < n_local && !issue_qk(n + 1)) break;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag))) break;
-      const uint32_t units = n0 + n < ts.nA ? 1u : 2u;
+      const uint32_t units = n < n_cached ? 1u : 2u;
+      // V rows of a canvas tile behind its last whole step of 32 keys were never written
+      const uint32_t keys = n < n_cached ? BLK : p.C - (n0 + n - ts.nA) * BLK;
       const uint32_t pt = tmem + T_S + (n & 1u) * 128u;
-      for (uint32_t i = 0; ok && i < units; ++i, ++uv) {
-        const uint32_t st = uv % cf::NV;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_V_FULL + st), (uv / cf::NV) & 1u, abort_flag));
+      for (uint32_t i = 0; i < units; ++i, ++uv) {
+        ok = __all_sync(0xffffffffu, i == 0 ? mbar_wait(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag)
+                                            : mbar_wait(bar(B_V2_FULL), (n - n_cached) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t vb = dv + uint64_t(st * (UNIT >> 4));
+          const uint32_t st = uv % cf::NV, vb = dv + st * (UNIT >> 4);
 #pragma unroll
           for (uint32_t ks = 0; ks < 4; ++ks) {
-            mma_ts(tmem + T_O, pt + ks * 8u, vb + ks * (4096u >> 4), IDESC_P1, (n | i | ks) != 0u);
-            mma_ts(tmem + T_O, pt + 32u + ks * 8u, vb + ks * (4096u >> 4), IDESC_P2, 1u);
+            if (ks != 0 && ks * 32u >= keys) break;
+            const uint32_t a = pt + (ks >> 1) * 64u + 32u + (ks & 1u) * 8u;
+            mma_ts(tmem + T_O, a, desc(vb + ks * (4096u >> 4)), IDESC_P1, ks == 0 ? (n | i) != 0u : 1u);
+            mma_ts(tmem + T_O, a + 16u, desc(vb + ks * (4096u >> 4)), IDESC_P2, 1u);
           }
           umma_commit(bar(B_V_EMPTY + st));
-          if (i + 1 == units) {
-            umma_commit(bar(B_PV + (n & 1u)));
-            if (n + 1 == n_local) umma_commit(bar(B_O));
-          }
+          if (n + 1 == n_local && i + 1 == units) umma_commit(bar(B_O));
         }
         __syncwarp();
       }
@@ -312,19 +346,21 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
   }
 
   // ------------------------------------------------------------------ output (softmax warps)
-  if (warp < cf::SM_WARPS) {
+  if (warp < SM_WARPS) {
     bool have = __all_sync(0xffffffffu, n_local > 0 && !*abort_flag);
     if (have) {
       have = __all_sync(0xffffffffu, mbar_wait(bar(B_O), 0u, abort_flag));
       tc_fence_after();
     }
-    // the row's sum is its threads' sums
-    bar_sync_quarter<32 * PARTS>(quarter);
-    xch[part * BLK + r] = l_run;
-    bar_sync_quarter<32 * PARTS>(quarter);
-    float l = xch[r];
-#pragma unroll
-    for (uint32_t i = 1; i < PARTS; ++i) l += xch[i * BLK + r];
+    // the row's sum is its four threads' sums, at the last reference
+    float* xl = xch;
+    const bool any = n_local > 0 && mt * BLK + quarter * 32u < rows_per_head;
+    bar_sync_id(9u + quarter, 128u);
+    const float m_row = any ? ref[r] : -INFINITY;
+    l_run = m_row == m_used ? l_run : (m_used == -INFINITY ? 0.f : l_run * fast_exp2(m_used - m_row));
+    xl[(grp * 2u + part) * BLK + r] = l_run;
+    bar_sync_id(9u + quarter, 128u);
+    const float l = (xl[r] + xl[BLK + r]) + (xl[2 * BLK + r] + xl[3 * BLK + r]);
     const bool direct = sq.n_splits == 1;
     const float mul = direct ? (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) : 1.0f;   // a sum that is NaN stays one
     const uint32_t t_lane = tmem + ((quarter * 32u) << 16);
@@ -341,8 +377,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
                         : (size_t(blockIdx.x) * BLK + rk) * 256u;
     }
 #pragma unroll 1
-    for (uint32_t cc = 0; cc < cf::OCOLS / 32; ++cc) {
-      const uint32_t col = part * cf::OCOLS + cc * 32u;
+    for (uint32_t cc = 0; cc < 2; ++cc) {
+      const uint32_t col = (grp * 2u + part) * 64u + cc * 32u;
       uint32_t o[32];
       if (have) {
         tmem_ld32(t_lane + T_O + col, o);
@@ -370,35 +406,38 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) dg_kv8_attn_kernel(const _
       __syncwarp();
     }
     const uint32_t R = mt * BLK + r;
-    if (part == 0 && R < rows_per_head) {
+    if (part == 0 && grp == 0 && R < rows_per_head) {
       if (!direct)
-        p.ws_ml[size_t(blockIdx.x) * BLK + r] = make_float2(m_used, l);
+        p.ws_ml[size_t(blockIdx.x) * BLK + r] = make_float2(m_row, l);
       else if (p.lse != nullptr && z == 0)
         p.lse[(size_t(b) * p.C + R / p.G) * p.Hq + kvh * p.G + R % p.G] =
-            l == 0.f ? -INFINITY : (m_used - LIFT + log2f(l)) * 0.6931471805599453f;
+            l == 0.f ? -INFINITY : (m_row - LIFT + log2f(l)) * 0.6931471805599453f;
     }
   }
 
   if (*abort_flag) {
     if (tid == 0) dev_status_set(p.status, DG_DEV_WAIT_TIMEOUT, KID_ATTN, blockIdx.x, n_local);
-    if (warp == cf::W_K && lane == 0) {
+    if (warp == W_K && lane == 0) {
       const long long c0 = clock64();
       while (clock64() - c0 < 2000000ll) {}   // ~1 ms: far longer than any load in flight
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == cf::W_MMA) tmem_dealloc(tmem, 512);
+  if (warp == W_MMA) tmem_dealloc(tmem, 512);
 }
 
-// Splits of a row joined: a warp per row and 256 columns, the splits in order.  A split without keys has m = -inf.
+// Splits of a row joined: a row's 256 columns by WARPS warps, each a run of the splits in order, then the warps in order.  One
+// warp a row where the splits are few (and the rows many), eight where they are many.  A split without keys has m = -inf.
+template <uint32_t WARPS>
 __global__ void __launch_bounds__(256) dg_kv8_merge_kernel(const __grid_constant__ AttnParams8 p) {
+  __shared__ float part[8][264];
   grid_launch_dependents();
   grid_wait();
-  const uint32_t lane = threadIdx.x & 31u, b = blockIdx.y, KU = p.D / 256u;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, w = warp % WARPS, b = blockIdx.y, KU = p.D / 256u;
   const Seq& sq = p.seq[b];
-  const uint32_t x = blockIdx.x * 8u + (threadIdx.x >> 5);
-  if (sq.n_splits == 1 || x >= p.C * p.Hq * KU) return;
+  const uint32_t x = blockIdx.x * (8u / WARPS) + warp / WARPS;
+  if (sq.n_splits == 1 || x >= p.C * p.Hq * KU) return;      // (whole CTAs where warps work together)
   const uint32_t z = x % KU, row = x / KU, i = row / p.Hq, h = row % p.Hq, kvh = h / p.G;
   const uint32_t R = i * p.G + h % p.G, mt = R / BLK, r = R % BLK, S = sq.n_splits;
   const uint32_t stride = p.Hkv * p.MT * KU, first = sq.first_cta + (kvh * p.MT + mt) * KU + z;
@@ -407,24 +446,41 @@ __global__ void __launch_bounds__(256) dg_kv8_merge_kernel(const __grid_constant
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const uint32_t s1 = (w + 1) * S / WARPS;
 #pragma unroll 4
-  for (uint32_t s = 0; s < S; ++s) {
+  for (uint32_t s = w * S / WARPS; s < s1; ++s) {
     const size_t at = size_t(first + s * stride) * BLK + r;
     const float2 ml = p.ws_ml[at];
     const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * 256u + lane * 8u);
     const float4 a = src[0], c = src[1];
     if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float w = fast_exp2(ml.x - m);
-    l = fmaf(w, ml.y, l);
-    acc[0] = fmaf(w, a.x, acc[0]); acc[1] = fmaf(w, a.y, acc[1]); acc[2] = fmaf(w, a.z, acc[2]); acc[3] = fmaf(w, a.w, acc[3]);
-    acc[4] = fmaf(w, c.x, acc[4]); acc[5] = fmaf(w, c.y, acc[5]); acc[6] = fmaf(w, c.z, acc[6]); acc[7] = fmaf(w, c.w, acc[7]);
+    const float f = fast_exp2(ml.x - m);
+    l = fmaf(f, ml.y, l);
+    acc[0] = fmaf(f, a.x, acc[0]); acc[1] = fmaf(f, a.y, acc[1]); acc[2] = fmaf(f, a.z, acc[2]); acc[3] = fmaf(f, a.w, acc[3]);
+    acc[4] = fmaf(f, c.x, acc[4]); acc[5] = fmaf(f, c.y, acc[5]); acc[6] = fmaf(f, c.z, acc[6]); acc[7] = fmaf(f, c.w, acc[7]);
   }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
   const size_t orow = (size_t(b) * p.C + i) * p.Hq + h;
-  *reinterpret_cast<uint4*>(p.out + orow * p.D + z * 256u + lane * 8u) =
-      make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
-                 pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
-  if (p.lse != nullptr && z == 0 && lane == 0) p.lse[orow] = l == 0.f ? -INFINITY : (m - LIFT + log2f(l)) * 0.6931471805599453f;
+  if (WARPS > 1) {
+    *reinterpret_cast<float4*>(&part[warp][lane * 8u]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<float4*>(&part[warp][lane * 8u + 4u]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    if (lane == 0) part[warp][256] = l;
+    __syncthreads();
+    l = 0.f;
+    float y = 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < WARPS; ++k) {
+      l += part[k][256];
+      y += part[k][threadIdx.x];
+    }
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+    p.out[orow * p.D + z * 256u + threadIdx.x] = __float2bfloat16(y * inv);
+  } else {
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+    *reinterpret_cast<uint4*>(p.out + orow * p.D + z * 256u + lane * 8u) =
+        make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                   pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+  }
+  if (p.lse != nullptr && z == 0 && w == 0 && lane == 0) p.lse[orow] = l == 0.f ? -INFINITY : (m - LIFT + log2f(l)) * 0.6931471805599453f;
 }
 
 cudaError_t configure_attn() {
@@ -436,7 +492,7 @@ cudaError_t configure_attn() {
 cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_ctas);
-  cfg.blockDim = dim3(p.D == 256 ? Cfg<256>::THREADS : Cfg<512>::THREADS);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = p.D == 256 ? Cfg<256>::SMEM : Cfg<512>::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -446,10 +502,15 @@ cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t mos
   cfg.numAttrs = 1;
   cudaError_t e = p.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<512>, p);
   if (e != cudaSuccess || most_splits == 1) return e;
-  cfg.gridDim = dim3((p.C * p.Hq * (p.D / 256u) + 7u) / 8u, p.n_seq);
+  const uint32_t rows = p.C * p.Hq * (p.D / 256u);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel, p);
+  if (most_splits > 4) {
+    cfg.gridDim = dim3(rows, p.n_seq);
+    return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<8>, p);
+  }
+  cfg.gridDim = dim3((rows + 7u) / 8u, p.n_seq);
+  return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<1>, p);
 }
 
 }  // namespace kv8

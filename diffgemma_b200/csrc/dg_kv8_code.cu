@@ -34,7 +34,7 @@ __device__ __forceinline__ float row_rsqrt(float x) { return rsqrtf(x); }
 __device__ __forceinline__ double row_rsqrt(double x) { return rsqrt(x); }
 
 // Warp-wide: a head's row, lane l holding elements [8 (l + 32 j), + 8).  RMS norm with weight w (null: unit; norm = false:
-// none) and rotation by `tab` (null: none); the result as bf16 pairs.
+// none) and rotation by `tab` (null: none; laid out by angles()); the result as bf16 pairs.
 template <class T, int NJ>
 __device__ __forceinline__ void row_to_bf16(const uint4 (&raw)[NJ], const __nv_bfloat16* w, bool norm, float eps, const Rope& rope,
                                             const typename Pair<T>::type* tab, uint32_t lane, uint4 (&out)[NJ]) {
@@ -82,7 +82,7 @@ __device__ __forceinline__ void row_to_bf16(const uint4 (&raw)[NJ], const __nv_b
       const bool first = c < hc, second = c >= dc && c < dc + hc;
       rot[j] = first || second;
       src[j] = first ? c + dc : (second ? c - dc : c);
-      base[j] = 8u * (first ? c : (second ? c - dc : 0u));
+      base[j] = first ? c : (second ? c - dc : 0u);
       sign[j] = first ? T(-1) : T(1);
     }
 #pragma unroll
@@ -94,7 +94,7 @@ __device__ __forceinline__ void row_to_bf16(const uint4 (&raw)[NJ], const __nv_b
           const T far = __shfl_sync(0xffffffffu, x[NJ - 1][i], int(src[j] & 31u));
           if (src[j] >= 32u) other = far;
         }
-        const typename Pair<T>::type cs = tab[base[j] + i];
+        const typename Pair<T>::type cs = tab[i * hc + base[j]];
         y[j][i] = rot[j] ? fma(other, sign[j] * cs.y, x[j][i] * cs.x) : x[j][i];
       }
 #pragma unroll
@@ -144,162 +144,196 @@ struct PosList {
   uint64_t pos[MAX_SEQ];
 };
 
-// (cos, sin) of PASS tokens from `first` on: tab[token][half].  The angles of a thread's tokens are reached by rotation
-// (64 bits: 1e-15 after a block), one table look-up of three angles for a block.
+// (cos, sin) of n_tok <= PASS tokens from `first` on: tab[token][8][half / 8], pair d at [d % 8][d / 8], so that the lanes of a
+// warp, eight pairs each, read neighbours.  A thread's tokens follow one another: two look-ups of
+// an angle, the others by rotation (64 bits: 1e-15 after a block).  Groups of half threads; every thread of the CTA calls.
 template <class T>
-struct Angles {
-  double2 z, one, pass;
-  uint32_t d, g, per;
-  bool on;
-  __device__ __forceinline__ void start(const Rope& r, double first) {
-    const uint32_t groups = r.half ? CT / r.half : 1u;
-    per = (PASS + groups - 1u) / groups;
-    d = r.half ? threadIdx.x % r.half : 0u;
-    g = r.half ? threadIdx.x / r.half : 0u;
-    on = r.half != 0u && g < groups && g * per < PASS;
-    if (on) {
-      const double t = turns_of(r, d);
-      z = unit_at(first + double(g * per), t);
-      one = unit_at(1.0, t);
-      pass = unit_at(double(PASS), t);
-    }
+__device__ __forceinline__ void angles(const Rope& r, double first, uint32_t n_tok, typename Pair<T>::type* tab) {
+  const uint32_t groups = CT / r.half, per = (n_tok + groups - 1u) / groups;
+  const uint32_t d = threadIdx.x % r.half, t0 = threadIdx.x / r.half * per;
+  if (threadIdx.x >= groups * r.half || t0 >= n_tok) return;
+  const double turns = turns_of(r, d);
+  double2 z = unit_at(first + double(t0), turns), one = make_double2(1.0, 0.0);
+  if (per > 1u) one = unit_at(1.0, turns);
+  for (uint32_t j = 0; j < per && t0 + j < n_tok; ++j) {
+    typename Pair<T>::type o;
+    o.x = T(z.x);
+    o.y = T(z.y);
+    tab[(t0 + j) * r.half + (d & 7u) * (r.half >> 3) + (d >> 3)] = o;
+    z = cmul(z, one);
   }
-  __device__ __forceinline__ void fill(const Rope& r, typename Pair<T>::type* tab) {
-    if (!on) return;
-    double2 c = z;
-    for (uint32_t j = 0; j < per && g * per + j < PASS; ++j) {
-      typename Pair<T>::type o;
-      o.x = T(c.x);
-      o.y = T(c.y);
-      tab[(g * per + j) * r.half + d] = o;
-      c = cmul(c, one);
-    }
-    z = cmul(z, pass);
-  }
-};
-
-// The rows of one block of 128 tokens of one head, K or V: in registers as bf16, 8 rows a warp (row = 16 pass + warp).
-// row(r) says where row r comes from.  Returns the largest magnitude of the block.
-template <class T, int NJ, class Row>
-__device__ __forceinline__ float block_rows(const CodeParams& p, bool is_k, double first_pos, uint32_t n_rows, Row row, uint4 (&held)[8][NJ],
-                                            uint8_t* smem, float* red, bool* bad) {
-  typedef typename Pair<T>::type T2;
-  T2* tab = reinterpret_cast<T2*>(smem);
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const bool turn = is_k && !p.ready && p.rope.half != 0;
-  const bool norm = !p.ready && (is_k || p.v_norm);
-  Angles<T> ang;
-  if (turn) ang.start(p.rope, first_pos);
-  uint32_t top = 0;
-#pragma unroll
-  for (uint32_t s = 0; s < 8; ++s) {
-    uint4 raw[NJ];
-    const uint32_t r = s * PASS + warp;
-    const bool live = r < n_rows;
-    bool fresh = false;
-    if (live) fresh = row(r, raw);
-    if (s * PASS < n_rows && turn) {
-      __syncthreads();
-      ang.fill(p.rope, tab);
-      __syncthreads();
-    }
-    if (!live) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) held[s][j] = make_uint4(0u, 0u, 0u, 0u);
-      continue;
-    }
-    if (fresh) {
-      if (turn || norm)
-        row_to_bf16<T, NJ>(raw, is_k ? p.kw : nullptr, norm, p.eps, p.rope, turn ? tab + warp * p.rope.half : nullptr, lane, held[s]);
-      else {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) held[s][j] = raw[j];
-      }
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        uint4& h = held[s][j];
-        h = make_uint4(finite_or_zero(h.x, bad), finite_or_zero(h.y, bad), finite_or_zero(h.z, bad), finite_or_zero(h.w, bad));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) held[s][j] = raw[j];
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) top = abs_max2(abs_max2(abs_max2(abs_max2(top, held[s][j].x), held[s][j].y), held[s][j].z), held[s][j].w);
-  }
-  float t = fmaxf(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-  __syncthreads();
-  if (lane == 0) red[warp] = t;
-  __syncthreads();
-  t = red[lane & 15u];
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-  return t;
 }
 
 // ------------------------------------------------------------------------------------------- rows of a step
-// CTAs [0, canvas CTAs): (sequence, head, tile of 128 canvas tokens, K or V).  The others: one canvas token each, all its
-// query heads (the angles are computed once for all of them), and the rows behind the last token of a row tile as zeros.
+// A warp takes one row.  Canvas K and V: the rows of one (head, tile, K or V) share a scale; they lie in `slots` neighbouring
+// warps (up to 16 canvas tokens) or in the CTAs of a cluster, 16 tokens each, whose maxima meet over distributed shared memory.
+// Queries: a CTA for each canvas token, all heads (the angles are computed once for all of them).
+struct RowsPlan {
+  uint32_t slots, cluster;             // warps of a scale group in a CTA; CTAs of one (16 slots)
+  uint32_t canvas_ctas, per_seq;       // CTAs of canvas rows; of them, of a sequence
+  uint32_t heads;                      // KV heads that a CTA of 16 slots takes one after the other
+  uint32_t q_tokens, q_ctas;           // query CTAs of a sequence, of all
+};
+constexpr uint32_t ROW_HEADS = 4;
+
+__device__ __forceinline__ float max_of_halves(uint32_t two) {
+  return fmaxf(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+}
+
+// One row of canvas K or V: normed, rotated, rounded, what is not finite as zero.  Returns its largest magnitude.
 template <int NJ>
-__global__ void __launch_bounds__(CT, 1) dg_kv8_rows_kernel(const __grid_constant__ QueryParams q, const __grid_constant__ CodeParams p,
-                                                            const __grid_constant__ PosList pos, uint32_t canvas_ctas, uint32_t q_tokens) {
+__device__ __forceinline__ float canvas_row(const CodeParams& p, bool is_k, const uint4 (&raw)[NJ], const double2* tab, uint32_t lane, uint4 (&v)[NJ],
+                                            bool* bad) {
+  if (is_k || p.v_norm)
+    row_to_bf16<double, NJ>(raw, is_k ? p.kw : nullptr, true, p.eps, p.rope, is_k && p.rope.half != 0u ? tab : nullptr, lane, v);
+  else {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) v[j] = raw[j];
+  }
+  uint32_t top2 = 0;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    v[j] = make_uint4(finite_or_zero(v[j].x, bad), finite_or_zero(v[j].y, bad), finite_or_zero(v[j].z, bad), finite_or_zero(v[j].w, bad));
+    top2 = abs_max2(abs_max2(abs_max2(abs_max2(top2, v[j].x), v[j].y), v[j].z), v[j].w);
+  }
+  float top = max_of_halves(top2);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return top;
+}
+// Stores row r of a canvas tile of `valid` tokens as two terms, and zeros behind V's last row up to a whole step of 32 keys
+// (their weights are zero, and zero times NaN is not); rows r, r + stride, ...
+template <int NJ>
+__device__ __forceinline__ void store_canvas_row(const CodeParams& p, bool is_k, size_t tile, uint32_t r, uint32_t stride, uint32_t valid, float top,
+                                                 uint32_t lane, const uint4 (&v)[NJ]) {
+  constexpr uint32_t D = 256u * NJ;
+  const int e = scale_exp(top);
+  const float mul = pow2i(-e);
+  uint8_t* dst = (is_k ? p.k_codes : p.v_codes) + tile * 2u * BLK * D;
+  const uint32_t end = is_k ? valid : (valid + 31u) / 32u * 32u;
+  for (uint32_t x = r; x < end; x += stride) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const uint32_t off = code8_off(x, lane + 32u * j);
+      uint2 c = make_uint2(0u, 0u), rest = c;
+      if (x < valid) c = code8(v[j], mul, &rest);
+      *reinterpret_cast<uint2*>(dst + off) = c;
+      *reinterpret_cast<uint2*>(dst + BLK * D + off) = rest;
+    }
+  }
+  if (lane == 0 && r == 0) (is_k ? p.k_exp : p.v_exp)[tile] = e;
+}
+
+template <int NJ>
+__global__ void __launch_bounds__(CT, NJ == 1 ? 2 : 1) dg_kv8_rows_kernel(const __grid_constant__ QueryParams q, const __grid_constant__ CodeParams p,
+                                                                         const __grid_constant__ PosList pos, const __grid_constant__ RowsPlan plan) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float red[16];
+  __shared__ float red[ROW_HEADS][16];
   grid_launch_dependents();
   grid_wait();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   constexpr uint32_t D = 256u * NJ;
-  if (blockIdx.x < canvas_ctas) {
-    uint32_t x = blockIdx.x;
-    const bool is_k = (x & 1u) == 0u;
-    x >>= 1;
-    const uint32_t ct = x % p.n_ctiles;
-    x /= p.n_ctiles;
-    const uint32_t h = x % p.Hkv, b = x / p.Hkv;
-    const uint32_t t0 = ct * BLK, n_rows = p.n - t0 < BLK ? p.n - t0 : BLK;
-    const __nv_bfloat16* src = (is_k ? p.k : p.v) + (size_t(b) * p.n + t0) * p.Hkv * D + size_t(h) * D;
-    uint4 held[8][NJ];
+  double2* tab = reinterpret_cast<double2*>(smem);
+  if (blockIdx.x < plan.canvas_ctas && plan.slots < 16u) {
+    // few tokens: the warps are (head, K or V, token)
+    const uint32_t b = blockIdx.x / plan.per_seq, g = blockIdx.x % plan.per_seq * (16u / plan.slots) + warp / plan.slots;
+    const uint32_t t = warp % plan.slots, h = g >> 1;
+    const bool on = h < p.Hkv, is_k = (g & 1u) == 0u, live = on && t < p.n;
+    const __nv_bfloat16* src = (is_k ? p.k : p.v) + ((size_t(b) * p.n + t) * p.Hkv + h) * D + 8u * lane;
+    uint4 raw[NJ], v[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) raw[j] = live ? *reinterpret_cast<const uint4*>(src + 256u * j) : make_uint4(0u, 0u, 0u, 0u);
+    if (p.rope.half != 0u) angles<double>(p.rope, double(pos.pos[b]), p.n, tab);
+    __syncthreads();
     bool bad = false;
-    const float top = block_rows<double, NJ>(
-        p, is_k, double(pos.pos[b]) + double(t0), n_rows,
-        [&](uint32_t r, uint4 (&raw)[NJ]) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + size_t(r) * p.Hkv * D + 8u * (lane + 32u * j));
-          return true;
-        },
-        held, smem, red, &bad);
-    const int e = scale_exp(top);
-    const float mul = pow2i(-e);
-    const size_t tile = (size_t(b) * p.Hkv + h) * p.n_ctiles + ct;
-    uint8_t* dst = (is_k ? p.k_codes : p.v_codes) + tile * 2u * BLK * D;
-#pragma unroll
-    for (uint32_t s = 0; s < 8; ++s)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint32_t off = code8_off(s * PASS + warp, lane + 32u * j);
-        uint2 rest;
-        const uint2 c = code8(held[s][j], mul, &rest);
-        *reinterpret_cast<uint2*>(dst + off) = c;
-        *reinterpret_cast<uint2*>(dst + BLK * D + off) = rest;
-      }
-    if (threadIdx.x == 0) (is_k ? p.k_exp : p.v_exp)[tile] = e;
-    if (bad) dev_status_set(p.status, DG_DEV_NOT_FINITE, KID_CODE, blockIdx.x, t0);
+    const float mine = live ? canvas_row<NJ>(p, is_k, raw, tab + t * p.rope.half, lane, v, &bad) : 0.f;
+    if (lane == 0) red[0][warp] = mine;
+    __syncthreads();
+    float top = 0.f;
+    for (uint32_t i = 0; i < plan.slots; ++i) top = fmaxf(top, red[0][warp / plan.slots * plan.slots + i]);
+    if (on) store_canvas_row<NJ>(p, is_k, size_t(b) * p.Hkv + h, t, plan.slots, p.n, top, lane, v);
+    if (bad) dev_status_set(p.status, DG_DEV_NOT_FINITE, KID_CODE, blockIdx.x, t);
     return;
   }
-  const uint32_t x = blockIdx.x - canvas_ctas;
-  const uint32_t b = x / q_tokens, i = x % q_tokens;
+  if (blockIdx.x < plan.canvas_ctas) {
+    // a cluster: (sequence, run of heads, tile, K or V); a CTA 16 tokens, a warp one of them in every head of the run
+    const uint32_t rank = blockIdx.x % plan.cluster;
+    uint32_t x = blockIdx.x / plan.cluster;
+    const uint32_t b = x / plan.per_seq;
+    x %= plan.per_seq;
+    const bool is_k = (x & 1u) == 0u;
+    const uint32_t ct = (x >> 1) % p.n_ctiles, h0 = (x >> 1) / p.n_ctiles * plan.heads;
+    const uint32_t r = rank * 16u + warp, t = ct * BLK + r;
+    const bool live = t < p.n;
+    const __nv_bfloat16* src = (is_k ? p.k : p.v) + ((size_t(b) * p.n + t) * p.Hkv + h0) * D + 8u * lane;
+    uint4 v[ROW_HEADS][NJ];
+#pragma unroll
+    for (uint32_t i = 0; i < ROW_HEADS; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        v[i][j] = live && i < plan.heads && h0 + i < p.Hkv ? *reinterpret_cast<const uint4*>(src + size_t(i) * D + 256u * j) : make_uint4(0u, 0u, 0u, 0u);
+    if (is_k && p.rope.half != 0u) {
+      const uint32_t first = ct * BLK + rank * 16u;
+      if (first < p.n) angles<double>(p.rope, double(pos.pos[b]) + double(first), p.n - first < 16u ? p.n - first : 16u, tab);
+      __syncthreads();
+    }
+    bool bad = false;
+#pragma unroll
+    for (uint32_t i = 0; i < ROW_HEADS; ++i) {
+      if (i >= plan.heads) continue;
+      float mine = 0.f;
+      if (live) {
+        uint4 y[NJ];
+        mine = canvas_row<NJ>(p, is_k, v[i], tab + warp * p.rope.half, lane, y, &bad);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) v[i][j] = y[j];
+      }
+      if (lane == 0) red[i][warp] = mine;
+    }
+    float top[ROW_HEADS] = {};
+    if (plan.cluster > 1u) {
+      cluster_sync_all();
+#pragma unroll
+      for (uint32_t i = 0; i < ROW_HEADS; ++i) {
+        if (i >= plan.heads) continue;
+        const uint32_t at = smem_u32(&red[i][lane & 15u]);
+        for (uint32_t c = lane >> 4; c < plan.cluster; c += 2u) {
+          float y;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(dsmem_addr(at, c)) : "memory");
+          top[i] = fmaxf(top[i], y);
+        }
+      }
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (uint32_t i = 0; i < ROW_HEADS; ++i) top[i] = red[i][lane & 15u];
+    }
+    const uint32_t valid = p.n - ct * BLK < BLK ? p.n - ct * BLK : BLK;
+#pragma unroll
+    for (uint32_t i = 0; i < ROW_HEADS; ++i) {
+      if (i >= plan.heads || h0 + i >= p.Hkv) continue;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+      store_canvas_row<NJ>(p, is_k, (size_t(b) * p.Hkv + h0 + i) * p.n_ctiles + ct, r, 16u * plan.cluster, valid, top[i], lane, v[i]);
+    }
+    if (bad) dev_status_set(p.status, DG_DEV_NOT_FINITE, KID_CODE, blockIdx.x, t);
+    if (plan.cluster > 1u) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves while its maxima may be read
+    return;
+  }
+  if (blockIdx.x >= plan.canvas_ctas + plan.q_ctas) return;      // the grid is a whole number of clusters
+  const uint32_t x = blockIdx.x - plan.canvas_ctas;
+  const uint32_t b = x / plan.q_tokens, i = x % plan.q_tokens;
   const QueryRows& o = q.rows;
-  double2* tab = reinterpret_cast<double2*>(smem);
-  if (!q.prenormed && i < o.C && threadIdx.x < q.rope.half)
-    tab[threadIdx.x] = unit_at(double(pos.pos[b]) + double(i), turns_of(q.rope, threadIdx.x));
-  __syncthreads();
+  const bool live = i < o.C;
+  if (live && q.rope.half != 0u) {
+    angles<double>(q.rope, double(pos.pos[b]) + double(i), 1u, tab);
+    __syncthreads();
+  }
   for (uint32_t h = warp; h < o.Hq; h += CT / 32u) {
     const uint32_t kvh = h / o.G, R = i * o.G + h % o.G;
     if (R >= o.MT * BLK) continue;
     uint4 v[NJ];
-    const bool live = i < o.C;
     if (live) {
       const size_t at = ((size_t(b) * o.C + i) * o.Hq + h) * D + 8u * lane;
       uint4 raw[NJ];
@@ -322,12 +356,8 @@ __global__ void __launch_bounds__(CT, 1) dg_kv8_rows_kernel(const __grid_constan
     uint32_t top2 = 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) top2 = abs_max2(abs_max2(abs_max2(abs_max2(top2, v[j].x), v[j].y), v[j].z), v[j].w);
-    uint32_t top = top2 > 0xffffu && (top2 >> 16) > (top2 & 0xffffu) ? top2 >> 16 : top2 & 0xffffu;
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, top, m);
-      top = other > top ? other : top;
-    }
+    uint32_t top = (top2 >> 16) > (top2 & 0xffffu) ? top2 >> 16 : top2 & 0xffffu;
+    top = __reduce_max_sync(0xffffffffu, top);
     // a row that is not finite has no scores: its codes are NaN
     const bool fin = top < 0x7f80u;
     const int e = fin ? scale_exp(__uint_as_float(top << 16)) : 0;
@@ -354,17 +384,23 @@ __global__ void __launch_bounds__(CT, 1) dg_kv8_rows_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------- append
-// One CTA for each (block, head, K or V) that the new tokens touch.  The first block may hold tokens already: their values
-// are read, and the block is coded as a whole at the scale that all of it needs.
+// One CTA (head_dim 512: a cluster of two, 64 tokens each) for each (block, head, K or V) that the new tokens touch; the rows
+// are in registers from load to store, 16-byte chunks of 8 / NJ rows a warp, two CTAs an SM: one loads while the other works.
+// The first block may hold tokens already: their values are read, and the block is coded as a whole at the scale that all
+// of it needs.  The angles of 32 tokens at a time: a thread's pair turns from pass to pass in 64 bits, within one in 32.
+constexpr uint32_t APASS = 32;
+
 template <int NJ>
-__global__ void __launch_bounds__(CT, 1) dg_kv8_append_kernel(const __grid_constant__ CodeParams p) {
+__global__ void __launch_bounds__(CT, 2) dg_kv8_append_kernel(const __grid_constant__ CodeParams p) {
+  constexpr uint32_t D = 256u * NJ, RW = 8u / NJ, TOK = 16u * RW;     // rows of a warp, tokens of a CTA
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[16];
+  float2* tab = reinterpret_cast<float2*>(smem);
   grid_launch_dependents();
   grid_wait();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  constexpr uint32_t D = 256u * NJ;
-  uint32_t x = blockIdx.x;
+  uint32_t x = blockIdx.x / NJ;
+  const uint32_t rank = blockIdx.x % NJ;
   const bool is_k = (x & 1u) == 0u;
   x >>= 1;
   const uint32_t h = x % p.Hkv, blk = p.n_keys / BLK + x / p.Hkv;
@@ -373,41 +409,108 @@ __global__ void __launch_bounds__(CT, 1) dg_kv8_append_kernel(const __grid_const
   const uint32_t n_rows = end - t0 < BLK ? end - t0 : BLK;
   uint8_t* codes = (is_k ? p.k_codes : p.v_codes) + (size_t(h) * p.blocks + blk) * BLK * D;
   int32_t* exps = (is_k ? p.k_exp : p.v_exp) + size_t(h) * p.blocks + blk;
-  const float old = kept ? pow2i(*exps) : 1.0f;
   const __nv_bfloat16* src = is_k ? p.k : p.v;
-  uint4 held[8][NJ];
+  // row s of this warp
+  auto row = [&](uint32_t s) { return rank * TOK + (s >> 1) * APASS + warp * 2u + (s & 1u); };
+  uint4 held[RW][NJ];
+#pragma unroll
+  for (uint32_t s = 0; s < RW; ++s) {
+    const uint32_t r = row(s);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      held[s][j] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < n_rows && r >= kept)
+        held[s][j] = __ldcs(reinterpret_cast<const uint4*>(src + (size_t(t0 + r - p.n_keys) * p.Hkv + h) * D + 8u * (lane + 32u * j)));
+    }
+  }
+  if (kept != 0u) {
+    const float old = pow2i(*exps);
+#pragma unroll
+    for (uint32_t s = 0; s < RW; ++s) {
+      const uint32_t r = row(s);
+      if (r >= kept) continue;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint2 c = *reinterpret_cast<const uint2*>(codes + code8_off(r, lane + 32u * j));
+        const float2 a = f32x2_from_e4m3x2(uint16_t(c.x)), b = f32x2_from_e4m3x2(uint16_t(c.x >> 16));
+        const float2 f = f32x2_from_e4m3x2(uint16_t(c.y)), g = f32x2_from_e4m3x2(uint16_t(c.y >> 16));
+        held[s][j] = make_uint4(pack_bf16x2(a.x * old, a.y * old), pack_bf16x2(b.x * old, b.y * old),
+                                pack_bf16x2(f.x * old, f.y * old), pack_bf16x2(g.x * old, g.y * old));
+      }
+    }
+  }
+  const bool turn = is_k && !p.ready && p.rope.half != 0u, norm = !p.ready && (is_k || p.v_norm);
+  // a thread's pair and its run of the pass's tokens
+  const uint32_t groups = turn ? CT / p.rope.half : 1u, per = (APASS + groups - 1u) / groups;
+  const uint32_t dim = turn ? threadIdx.x % p.rope.half : 0u, tok = turn ? threadIdx.x / p.rope.half * per : APASS;
+  double2 z = {}, hop = {};
+  float2 one = {};
+  if (turn && threadIdx.x < groups * p.rope.half && tok < APASS) {
+    const double turns = turns_of(p.rope, dim);
+    z = unit_at(double(p.pos) + double(t0 + rank * TOK + tok) - double(p.n_keys), turns);
+    hop = unit_at(double(APASS), turns);
+    const double2 o = unit_at(1.0, turns);
+    one = make_float2(float(o.x), float(o.y));
+  }
   bool bad = false;
-  const float top = block_rows<float, NJ>(
-      p, is_k, double(p.pos) + double(t0) - double(p.n_keys), n_rows,
-      [&](uint32_t r, uint4 (&raw)[NJ]) {
-        if (r >= kept) {
-          const __nv_bfloat16* s = src + (size_t(t0 + r - p.n_keys) * p.Hkv + h) * D;
+  uint32_t top = 0;
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) raw[j] = *reinterpret_cast<const uint4*>(s + 8u * (lane + 32u * j));
-          return true;
+  for (uint32_t s = 0; s < RW; ++s) {
+    const uint32_t r = row(s);
+    if (turn && (s & 1u) == 0u) {
+      if (s != 0u) __syncthreads();
+      if (threadIdx.x < groups * p.rope.half) {
+        float2 c = make_float2(float(z.x), float(z.y));
+        for (uint32_t i = tok; i < tok + per && i < APASS; ++i) {
+          tab[i * p.rope.half + (dim & 7u) * (p.rope.half >> 3) + (dim >> 3)] = c;
+          c = make_float2(fmaf(c.x, one.x, -c.y * one.y), fmaf(c.x, one.y, c.y * one.x));
         }
+        z = cmul(z, hop);
+      }
+      __syncthreads();
+    }
+    if (r < n_rows && r >= kept) {
+      if (turn || norm) {
+        uint4 y[NJ];
+        row_to_bf16<float, NJ>(held[s], is_k ? p.kw : nullptr, norm, p.eps, p.rope, turn ? tab + (r % APASS) * p.rope.half : nullptr, lane, y);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const uint2 c = *reinterpret_cast<const uint2*>(codes + code8_off(r, lane + 32u * j));
-          const float2 a = f32x2_from_e4m3x2(uint16_t(c.x)), b = f32x2_from_e4m3x2(uint16_t(c.x >> 16));
-          const float2 f = f32x2_from_e4m3x2(uint16_t(c.y)), g = f32x2_from_e4m3x2(uint16_t(c.y >> 16));
-          raw[j] = make_uint4(pack_bf16x2(a.x * old, a.y * old), pack_bf16x2(b.x * old, b.y * old),
-                              pack_bf16x2(f.x * old, f.y * old), pack_bf16x2(g.x * old, g.y * old));
-        }
-        return false;
-      },
-      held, smem, red, &bad);
-  const int e = scale_exp(top);
+        for (int j = 0; j < NJ; ++j) held[s][j] = y[j];
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        uint4& y = held[s][j];
+        y = make_uint4(finite_or_zero(y.x, &bad), finite_or_zero(y.y, &bad), finite_or_zero(y.z, &bad), finite_or_zero(y.w, &bad));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) top = abs_max2(abs_max2(abs_max2(abs_max2(top, held[s][j].x), held[s][j].y), held[s][j].z), held[s][j].w);
+  }
+  float t = max_of_halves(top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+  if (lane == 0) red[warp] = t;
+  if (NJ == 1) {
+    __syncthreads();
+    t = red[lane & 15u];
+  } else {
+    cluster_sync_all();
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(t) : "r"(dsmem_addr(smem_u32(&red[lane & 15u]), lane >> 4)) : "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+  const int e = scale_exp(t);
   const float mul = pow2i(-e);
 #pragma unroll
-  for (uint32_t s = 0; s < 8; ++s) {
-    const uint32_t r = s * PASS + warp;
+  for (uint32_t s = 0; s < RW; ++s) {
+    const uint32_t r = row(s);
     if (r >= n_rows) continue;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) *reinterpret_cast<uint2*>(codes + code8_off(r, lane + 32u * j)) = code8(held[s][j], mul, nullptr);
   }
-  if (threadIdx.x == 0) *exps = e;
   if (bad) dev_status_set(p.status, DG_DEV_NOT_FINITE, KID_CODE, blockIdx.x, t0);
+  if (NJ > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves while its maximum may be read
+  if (threadIdx.x == 0 && rank == 0) *exps = e;                                     // (the other CTA has read the old scale)
 }
 
 // ------------------------------------------------------------------------------------------- read back
@@ -457,11 +560,12 @@ static cudaError_t launch(void (*fn)(A...), uint32_t grid, uint32_t threads, siz
   return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
-constexpr size_t ROWS_SMEM = PASS * 256u * sizeof(double2);   // angles of PASS tokens at the widest rotation
+constexpr size_t ROWS_SMEM = PASS * 256u * sizeof(double2);   // angles of PASS (append: APASS, in fp32) tokens at the widest rotation
 
 cudaError_t configure_code() {
   cudaError_t e = cudaSuccess;
-  for (const void* f : {reinterpret_cast<const void*>(dg_kv8_rows_kernel<1>), reinterpret_cast<const void*>(dg_kv8_rows_kernel<2>)})
+  for (const void* f : {reinterpret_cast<const void*>(dg_kv8_rows_kernel<1>), reinterpret_cast<const void*>(dg_kv8_rows_kernel<2>),
+                        reinterpret_cast<const void*>(dg_kv8_append_kernel<1>), reinterpret_cast<const void*>(dg_kv8_append_kernel<2>)})
     if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ROWS_SMEM));
   return e;
 }
@@ -469,16 +573,58 @@ cudaError_t configure_code() {
 cudaError_t launch_rows(const QueryParams& q, const CodeParams& p, const uint64_t* pos, uint32_t n_seq, cudaStream_t st) {
   PosList l = {};
   for (uint32_t b = 0; b < n_seq; ++b) l.pos[b] = pos[b];
-  const uint32_t canvas = n_seq * p.n_ctiles * q.rows.Hkv * 2u;
-  const uint32_t tokens = (q.rows.MT * BLK + q.rows.G - 1u) / q.rows.G;
-  const size_t smem = size_t(canvas ? PASS : 1u) * q.rope.half * sizeof(double2);
-  return launch(q.rows.D == 256 ? dg_kv8_rows_kernel<1> : dg_kv8_rows_kernel<2>, canvas + n_seq * tokens, CT, smem, st, q, p, l, canvas, tokens);
+  RowsPlan plan = {16, 1, 0, 1, 1, q.rows.C, 0};
+  if (p.n_ctiles != 0u) {
+    if (p.n <= 8u) {
+      plan.slots = 1;
+      while (plan.slots < p.n) plan.slots *= 2u;
+      plan.per_seq = (q.rows.Hkv * 2u + 16u / plan.slots - 1u) / (16u / plan.slots);
+      plan.canvas_ctas = n_seq * plan.per_seq;
+    } else {
+      const uint32_t tokens = p.n < BLK ? p.n : BLK;
+      while (plan.cluster * 16u < tokens) plan.cluster *= 2u;
+      plan.heads = q.rows.Hkv < ROW_HEADS ? q.rows.Hkv : ROW_HEADS;
+      plan.per_seq = (q.rows.Hkv + plan.heads - 1u) / plan.heads * p.n_ctiles * 2u;
+      plan.canvas_ctas = n_seq * plan.per_seq * plan.cluster;
+    }
+  }
+  // the key weights sum over whole row tiles: rows behind the last token are zeros there
+  if (q.lse != nullptr) plan.q_tokens = (q.rows.MT * BLK + q.rows.G - 1u) / q.rows.G;
+  plan.q_ctas = n_seq * plan.q_tokens;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((plan.canvas_ctas + plan.q_ctas + plan.cluster - 1u) / plan.cluster * plan.cluster);
+  cfg.blockDim = dim3(CT);
+  cfg.dynamicSmemBytes = size_t(p.n_ctiles ? plan.slots : 1u) * q.rope.half * sizeof(double2);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = plan.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return q.rows.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_rows_kernel<1>, q, p, l, plan) : cudaLaunchKernelEx(&cfg, dg_kv8_rows_kernel<2>, q, p, l, plan);
 }
 
 cudaError_t launch_append(const CodeParams& p, cudaStream_t st) {
-  const uint32_t blocks = (p.n_keys + p.n + BLK - 1u) / BLK - p.n_keys / BLK;
-  const size_t smem = p.ready ? 0 : size_t(PASS) * p.rope.half * sizeof(float2);
-  return launch(p.D == 256 ? dg_kv8_append_kernel<1> : dg_kv8_append_kernel<2>, blocks * p.Hkv * 2u, CT, smem, st, p);
+  const uint32_t blocks = (p.n_keys + p.n + BLK - 1u) / BLK - p.n_keys / BLK, nj = p.D / 256u;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks * p.Hkv * 2u * nj);
+  cfg.blockDim = dim3(CT);
+  cfg.dynamicSmemBytes = p.ready ? 0 : size_t(APASS) * p.rope.half * sizeof(float2);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = nj;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return nj == 1 ? cudaLaunchKernelEx(&cfg, dg_kv8_append_kernel<1>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_append_kernel<2>, p);
 }
 
 cudaError_t launch_read(const ReadParams& p, cudaStream_t st) {

@@ -1,17 +1,18 @@
 // Eviction: the n_recent last tokens of a cache and, of those before them, the n_keep - n_recent with the largest weights
 // (equal ones: lowest index), in order, into another cache.
 //
-// Selection, a cluster of eight CTAs for each head: the cut is found exactly by a radix over 32-bit order keys (digits of
-// 11, 11 and 10 bits; every CTA counts its eighth, the counts meet over distributed shared memory), then each thread places
-// its run of tokens by the counts ahead of it.  The weights are read from HBM once and then from L1 (64 KB a CTA at 131,072
-// tokens).  Moving, a CTA for each block of the new cache: 128 gathered rows of codes, whose values get the scale of their
-// new block; the codes stay as they are where the scale does.
+// Selection, a cluster of up to eight CTAs for each head: the cut is found exactly by a radix over 32-bit order keys (digits of
+// 11, 11 and 10 bits).  A thread holds its run of up to 16 tokens in registers (131,072 tokens a head; longer rows are read
+// again for each digit).  A CTA counts its part; of the digit's bins each CTA adds up an eighth over the cluster and stores the
+// sums to all (distributed shared memory carries every count once), then each finds the cut for itself, and each thread places
+// its run by the counts ahead of it.  Moving, a CTA for each block of the new cache: 128 gathered rows of codes, whose values
+// get the scale of their new block; the codes stay as they are where the scale does.
 #include "dg_kv8.cuh"
 
 namespace dg {
 namespace kv8 {
 
-constexpr uint32_t SEL_CTAS = 8, SEL_T = 1024, BINS = 2048, COPIES = 4;
+constexpr uint32_t SEL_T = 1024, BINS = 2048, RUN = 16;
 
 // larger key = larger weight; NaN below everything
 __device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : score_order_key(w); }
@@ -20,6 +21,9 @@ __device__ __forceinline__ uint32_t ld_dsmem(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ void st_dsmem(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // exclusive sum over the block of two counts
@@ -46,54 +50,68 @@ __device__ __forceinline__ uint2 block_scan2(uint2 v, uint2* warp_sum, uint2* to
   return make_uint2(bx + x.x - v.x, by + x.y - v.y);
 }
 
-__global__ void __cluster_dims__(SEL_CTAS, 1, 1) __launch_bounds__(SEL_T, 1) dg_kv8_select_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ uint32_t hist[COPIES][BINS];
-  __shared__ uint32_t mine[BINS];            // this CTA's counts, read by the others
+template <bool IN_REGS>
+__global__ void __launch_bounds__(SEL_T, 1) dg_kv8_select_kernel(const __grid_constant__ EvictParams p, uint32_t ctas) {
+  __shared__ uint32_t hist[BINS];            // this CTA's counts of a digit
+  __shared__ uint32_t sums[BINS];            // the cluster's
   __shared__ uint2 warp_sum[32];
   __shared__ uint32_t found[2];
   __shared__ uint32_t totals[2];             // kept and tied tokens of this CTA
   grid_launch_dependents();
   grid_wait();
-  const uint32_t tid = threadIdx.x, rank = cluster_ctarank(), h = blockIdx.x / SEL_CTAS;
+  const uint32_t tid = threadIdx.x, rank = blockIdx.x % ctas, h = blockIdx.x / ctas;
   const float* w = p.w + size_t(h) * p.ld;
   const uint32_t n = p.n_keys - p.n_recent, take = p.n_keep - p.n_recent;
-  const uint32_t seg = (n + SEL_CTAS - 1) / SEL_CTAS, per = (seg + SEL_T - 1) / SEL_T;
+  const uint32_t seg = (n + ctas - 1) / ctas, per = (seg + SEL_T - 1) / SEL_T;
   // this thread's run of tokens
   const uint32_t end_c = (rank + 1) * seg < n ? (rank + 1) * seg : n;
   uint32_t t0 = rank * seg + tid * per, t1 = t0 + per;
   if (t0 > end_c) t0 = end_c;
   if (t1 > end_c) t1 = end_c;
+  float run[IN_REGS ? RUN : 1];
+  if (IN_REGS) {
+#pragma unroll
+    for (uint32_t i = 0; i < RUN; ++i) run[i] = t0 + i < t1 ? __ldg(w + t0 + i) : 0.f;
+  }
+  // f(token, weight) for the tokens of the run, in order
+  auto each = [&](auto f) {
+    if (IN_REGS) {
+#pragma unroll
+      for (uint32_t i = 0; i < RUN; ++i)
+        if (t0 + i < t1) f(t0 + i, run[i]);
+    } else {
+      for (uint32_t t = t0; t < t1; ++t) f(t, __ldg(w + t));
+    }
+  };
+  auto sync_all = [&] {
+    if (ctas > 1) cluster_sync_all(); else __syncthreads();
+  };
 
   uint32_t prefix = 0, left = take;          // the digits found so far; tokens to take among those that share them
   if (take > 0) {
 #pragma unroll 1
     for (uint32_t pass = 0; pass < 3; ++pass) {
       const uint32_t shift = pass == 0 ? 21u : pass == 1 ? 10u : 0u, bits = pass == 2 ? 10u : 11u, bins = 1u << bits;
-      for (uint32_t i = tid; i < COPIES * BINS; i += SEL_T) (&hist[0][0])[i] = 0u;
+      hist[tid] = 0u;
+      hist[tid + SEL_T] = 0u;
       __syncthreads();
-      uint32_t* mh = hist[(tid >> 5) % COPIES];
-      for (uint32_t t = t0; t < t1; ++t) {
-        const uint32_t key = weight_key(__ldg(w + t));
-        if (pass == 0 || (key >> (shift + bits)) == prefix) atomicAdd(mh + ((key >> shift) & (bins - 1u)), 1u);
-      }
-      __syncthreads();
-      for (uint32_t i = tid; i < bins; i += SEL_T) {
-        uint32_t s = 0;
-#pragma unroll
-        for (uint32_t c = 0; c < COPIES; ++c) s += hist[c][i];
-        mine[i] = s;
-      }
-      cluster_sync_all();
-      // counts of the whole head, largest digit first: thread i has the bins bins - 1 - 2i and bins - 2 - 2i
-      uint32_t c0 = 0, c1 = 0;
-      if (2u * tid < bins) {
-        const uint32_t hi = smem_u32(mine) + (bins - 1u - 2u * tid) * 4u;
-#pragma unroll
-        for (uint32_t r = 0; r < SEL_CTAS; ++r) {
-          c0 += ld_dsmem(dsmem_addr(hi, r));
-          c1 += ld_dsmem(dsmem_addr(hi - 4u, r));
+      each([&](uint32_t, float x) {
+        const uint32_t key = weight_key(x);
+        if (pass == 0 || (key >> (shift + bits)) == prefix) atomicAdd(hist + ((key >> shift) & (bins - 1u)), 1u);
+      });
+      sync_all();
+      if (ctas > 1) {
+        for (uint32_t i = tid; i < bins / ctas; i += SEL_T) {
+          const uint32_t bin = rank * (bins / ctas) + i;
+          uint32_t s = 0;
+          for (uint32_t r = 0; r < ctas; ++r) s += ld_dsmem(dsmem_addr(smem_u32(hist + bin), r));
+          for (uint32_t r = 0; r < ctas; ++r) st_dsmem(dsmem_addr(smem_u32(sums + bin), r), s);
         }
+        cluster_sync_all();
       }
+      // largest digit first: thread i has the bins bins - 1 - 2i and bins - 2 - 2i
+      const uint32_t* src = ctas > 1 ? sums : hist;
+      const uint32_t c0 = 2u * tid < bins ? src[bins - 1u - 2u * tid] : 0u, c1 = 2u * tid < bins ? src[bins - 2u - 2u * tid] : 0u;
       uint2 total;
       const uint32_t before = block_scan2(make_uint2(c0 + c1, 0u), warp_sum, &total).x;
       if (before < left && left <= before + c0 + c1) {
@@ -101,7 +119,7 @@ __global__ void __cluster_dims__(SEL_CTAS, 1, 1) __launch_bounds__(SEL_T, 1) dg_
         found[0] = bins - 1u - 2u * tid - (in_first ? 0u : 1u);
         found[1] = left - before - (in_first ? 0u : c0);
       }
-      cluster_sync_all();                    // nobody writes `mine` again before all have read it; `found` is there
+      __syncthreads();
       prefix = (prefix << bits) | found[0];
       left = found[1];
     }
@@ -109,27 +127,29 @@ __global__ void __cluster_dims__(SEL_CTAS, 1, 1) __launch_bounds__(SEL_T, 1) dg_
   // kept: above the cut, and the first `left` of those at it
   uint32_t gt = 0, eq = 0;
   if (take > 0)
-    for (uint32_t t = t0; t < t1; ++t) {
-      const uint32_t key = weight_key(__ldg(w + t));
+    each([&](uint32_t, float x) {
+      const uint32_t key = weight_key(x);
       gt += key > prefix ? 1u : 0u;
       eq += key == prefix ? 1u : 0u;
-    }
+    });
   uint2 total;
   uint2 at = block_scan2(make_uint2(gt, eq), warp_sum, &total);
-  if (tid == 0) {
-    totals[0] = total.x;
-    totals[1] = total.y;
-  }
-  cluster_sync_all();
-  for (uint32_t r = 0; r < rank; ++r) {
-    at.x += ld_dsmem(dsmem_addr(smem_u32(&totals[0]), r));
-    at.y += ld_dsmem(dsmem_addr(smem_u32(&totals[1]), r));
+  if (ctas > 1) {
+    if (tid == 0) {
+      totals[0] = total.x;
+      totals[1] = total.y;
+    }
+    cluster_sync_all();
+    for (uint32_t r = 0; r < rank; ++r) {
+      at.x += ld_dsmem(dsmem_addr(smem_u32(&totals[0]), r));
+      at.y += ld_dsmem(dsmem_addr(smem_u32(&totals[1]), r));
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
   int32_t* kept = p.kept + size_t(h) * p.n_keep;
   float* w_out = p.w_out ? p.w_out + size_t(h) * p.ld_out : nullptr;
   if (take > 0)
-    for (uint32_t t = t0; t < t1; ++t) {
-      const float x = __ldg(w + t);
+    each([&](uint32_t t, float x) {
       const uint32_t key = weight_key(x);
       const bool tie = key == prefix;
       if (key > prefix || (tie && at.y < left)) {
@@ -139,12 +159,12 @@ __global__ void __cluster_dims__(SEL_CTAS, 1, 1) __launch_bounds__(SEL_T, 1) dg_
       }
       at.x += key > prefix ? 1u : 0u;
       at.y += tie ? 1u : 0u;
-    }
-  for (uint32_t i = rank * SEL_T + tid; i < p.n_recent; i += SEL_CTAS * SEL_T) {
+    });
+  for (uint32_t i = rank * SEL_T + tid; i < p.n_recent; i += ctas * SEL_T) {
     kept[take + i] = int32_t(n + i);
     if (w_out) w_out[take + i] = w[n + i];
   }
-  cluster_sync_all();                        // no CTA leaves while its counts may be read
+  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // no CTA leaves while its counts may be read
 }
 
 template <uint32_t D>
@@ -207,17 +227,26 @@ __global__ void __launch_bounds__(512) dg_kv8_move_kernel(const __grid_constant_
 }
 
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st) {
+  // CTAs of a head: one up to 4,096 tokens (four each thread), eight from 16,385
+  uint32_t ctas = 1;
+  while (ctas < 8 && (p.n_keys - p.n_recent) > ctas * 4u * SEL_T) ctas *= 2;
+  const bool in_regs = p.n_keys - p.n_recent <= ctas * SEL_T * RUN;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(SEL_CTAS * p.Hkv);
+  cfg.gridDim = dim3(ctas * p.Hkv);
   cfg.blockDim = dim3(SEL_T);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, dg_kv8_select_kernel, p);
+  cfg.numAttrs = 2;
+  const cudaError_t e = in_regs ? cudaLaunchKernelEx(&cfg, dg_kv8_select_kernel<true>, p, ctas) : cudaLaunchKernelEx(&cfg, dg_kv8_select_kernel<false>, p, ctas);
   if (e != cudaSuccess) return e;
+  cfg.numAttrs = 1;
   cfg.gridDim = dim3((p.n_keep + BLK - 1) / BLK, p.Hkv, 2);
   cfg.blockDim = dim3(512);
   return p.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_move_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_move_kernel<512>, p);
