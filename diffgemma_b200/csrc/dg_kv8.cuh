@@ -60,20 +60,31 @@ __device__ __forceinline__ uint32_t f16x2_from_e4m3x2(uint16_t v) {
   return r;
 }
 __device__ __forceinline__ float2 f32x2_from_e4m3x2(uint16_t v) { return unpack_f16x2(f16x2_from_e4m3x2(v)); }
-__device__ __forceinline__ uint16_t e4m3x2_from_f16x2(uint32_t v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ uint16_t e5m2x2_from_f16x2(uint32_t v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+// Four fp32 (v[0] in the low byte) to e4m3 or e5m2 with the bits of `r` added below the last kept one: a half for each of the
+// four, which rounds to nearest (ties away from zero).  Two of the four take their bits mirrored.  One instruction for four
+// numbers, where conversions by pairs are two each and a byte permutation.
+constexpr uint32_t RS_HALF = 0x80018001u;
+__device__ __forceinline__ uint32_t e4m3x4_half(float a, float b, float c, float d) {
   uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%4, %3, %2, %1}, %5;" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d), "r"(RS_HALF));
   return r;
+}
+__device__ __forceinline__ uint32_t e5m2x4_half(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("cvt.rs.satfinite.e5m2x4.f32 %0, {%4, %3, %2, %1}, %5;" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d), "r"(RS_HALF));
+  return r;
+}
+// x - h of an fp32 and an f16 number, in fp32
+__device__ __forceinline__ float sub_f32_f16(float x, uint16_t h) {
+  float r;
+  asm("{\n\t.reg .b16 m;\n\tmov.b16 m, 0xBC00;\n\tfma.rn.f32.f16 %0, %1, m, %2;\n\t}" : "=f"(r) : "h"(h), "f"(x));
+  return r;
+}
+// Four weights as e4m3 + e5m2: within 2^-8 of a weight down to 2^-6, within 2^-17 below
+__device__ __forceinline__ void split4(float a, float b, float c, float d, uint32_t* p1, uint32_t* p2) {
+  *p1 = e4m3x4_half(a, b, c, d);
+  const uint32_t lo = f16x2_from_e4m3x2(uint16_t(*p1)), hi = f16x2_from_e4m3x2(uint16_t(*p1 >> 16));
+  *p2 = e5m2x4_half(sub_f32_f16(a, uint16_t(lo)), sub_f32_f16(b, uint16_t(lo >> 16)), sub_f32_f16(c, uint16_t(hi)), sub_f32_f16(d, uint16_t(hi >> 16)));
 }
 
 // ---- tensor cores: kind::f8f6f4, fp32 accumulate.  A e4m3 (0) or e5m2 (1), B e4m3; other fields as for bf16.
@@ -107,6 +118,23 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst),
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
                : "memory");
+}
+// mbar_wait with its clock and the abort flag looked at every 64th poll only: a waiting warp shares its scheduler with warps that
+// compute, and a poll alone is a third of the instructions.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+#pragma unroll 1
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 0u) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > DG_WAIT_LIMIT_CYCLES) {
+        *abort_flag = 1u;
+        return false;
+      }
+    }
+  }
 }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -147,22 +175,20 @@ struct CodeParams {
   float eps;
   Rope rope;
   DevStatus* status;
-  // append: codes [Hkv][blocks][D / 128][128][128], exponents [Hkv][blocks]
+  // append: codes [Hkv][blocks][D / 128][128][128], exponents [Hkv][blocks][2] (K, V)
   uint8_t* k_codes;
   uint8_t* v_codes;
-  int32_t* k_exp;
-  int32_t* v_exp;
+  int32_t* exps;
   uint32_t blocks, n_keys;
   uint64_t pos;
-  // canvas: codes [seq][Hkv][2 tiles][2 terms][D / 128][128][128], exponents [seq][Hkv][2 tiles]; K first, V behind it
+  // canvas: codes [seq][Hkv][tiles][2 terms][D / 128][128][128], exponents [seq][Hkv][tiles][2]
   uint32_t n_ctiles;
 };
 
 struct Seq {                   // one cache of an attention launch
   const uint8_t* k;
   const uint8_t* v;
-  const int32_t* k_exp;
-  const int32_t* v_exp;
+  const int2* exps;
   uint32_t blocks;             // capacity in blocks: stride of a head
   uint32_t n_keys;
   uint32_t first_cta;          // CTAs of the sequences before it
@@ -178,8 +204,7 @@ struct AttnParams8 {
   const float2* q_row;
   const uint8_t* c_k;          // canvas codes
   const uint8_t* c_v;
-  const int32_t* c_kexp;
-  const int32_t* c_vexp;
+  const int2* c_exps;
   uint32_t n_ctiles;
   __nv_bfloat16* out;          // [seq][C][Hq][D]
   float* lse;                  // [seq][C][Hq] or null
@@ -192,7 +217,7 @@ struct WeightParams {
   const uint8_t* q_codes;
   const float2* q_row;
   const uint8_t* k;
-  const int32_t* k_exp;
+  const int2* exps;
   uint32_t blocks, n_keys;
   uint32_t C, Hkv, G, MT;
   uint32_t mode, windowed, wm1;
@@ -213,21 +238,18 @@ struct EvictParams {
   uint64_t ld_out;
   const uint8_t* k;
   const uint8_t* v;
-  const int32_t* k_exp;
-  const int32_t* v_exp;
+  const int32_t* exps;
   uint32_t blocks;
   uint8_t* to_k;
   uint8_t* to_v;
-  int32_t* to_kexp;
-  int32_t* to_vexp;
+  int32_t* to_exps;
   uint32_t to_blocks;
 };
 
 struct ReadParams {
   const uint8_t* k;
   const uint8_t* v;
-  const int32_t* k_exp;
-  const int32_t* v_exp;
+  const int32_t* exps;
   uint32_t blocks, Hkv, D, slot0, n;
   __nv_bfloat16* k_out;        // [n][Hkv][D]
   __nv_bfloat16* v_out;

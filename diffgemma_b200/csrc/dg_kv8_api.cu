@@ -27,8 +27,7 @@ struct dg_kv8 {
   int device = 0;
   uint8_t* k = nullptr;        // [Hkv][blocks][D / 128][128][128]
   uint8_t* v = nullptr;
-  int32_t* k_exp = nullptr;    // [Hkv][blocks]
-  int32_t* v_exp = nullptr;
+  int32_t* exps = nullptr;     // [Hkv][blocks][2]: exponents of the scales of K and V
   uint32_t blocks = 0, Hkv = 0, D = 0;
 };
 
@@ -80,13 +79,11 @@ extern "C" int32_t dg_kv8_create(dg_ctx* c, const dg_layer_desc* d, uint64_t cap
   const size_t tiles = size_t(kv->Hkv) * kv->blocks, bytes = tiles * BLK * kv->D;
   cudaError_t e = cudaMalloc(&kv->k, bytes);
   if (e == cudaSuccess) e = cudaMalloc(&kv->v, bytes);
-  if (e == cudaSuccess) e = cudaMalloc(&kv->k_exp, tiles * sizeof(int32_t));
-  if (e == cudaSuccess) e = cudaMalloc(&kv->v_exp, tiles * sizeof(int32_t));
+  if (e == cudaSuccess) e = cudaMalloc(&kv->exps, tiles * 2 * sizeof(int32_t));
   // whole blocks are read and masked afterwards: every code is a finite number from the start
   if (e == cudaSuccess) e = cudaMemsetAsync(kv->k, 0, bytes, c->stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(kv->v, 0, bytes, c->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(kv->k_exp, 0, tiles * sizeof(int32_t), c->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(kv->v_exp, 0, tiles * sizeof(int32_t), c->stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(kv->exps, 0, tiles * 2 * sizeof(int32_t), c->stream);
   if (e != cudaSuccess) {
     dg_kv8_destroy(kv);
     return fail_cuda(e, "dg_kv8_create");
@@ -103,8 +100,7 @@ extern "C" int32_t dg_kv8_destroy(dg_kv8* kv) {
   }
   cudaFree(kv->k);
   cudaFree(kv->v);
-  cudaFree(kv->k_exp);
-  cudaFree(kv->v_exp);
+  cudaFree(kv->exps);
   delete kv;
   return DG_OK;
 }
@@ -134,8 +130,7 @@ static int32_t append8(dg_ctx* c, const dg_layer_desc* d, dg_kv8* kv, uint64_t n
   p.status = c->d_status;
   p.k_codes = kv->k;
   p.v_codes = kv->v;
-  p.k_exp = kv->k_exp;
-  p.v_exp = kv->v_exp;
+  p.exps = kv->exps;
   p.blocks = kv->blocks;
   p.n_keys = uint32_t(n_keys);
   p.pos = pos;
@@ -184,8 +179,7 @@ extern "C" int32_t dg_kv8_read(dg_kv8* kv, void* k_out, void* v_out, uint64_t sl
   kv8::ReadParams p = {};
   p.k = kv->k;
   p.v = kv->v;
-  p.k_exp = kv->k_exp;
-  p.v_exp = kv->v_exp;
+  p.exps = kv->exps;
   p.blocks = kv->blocks;
   p.Hkv = kv->Hkv;
   p.D = kv->D;
@@ -205,7 +199,7 @@ namespace {
 
 // Workspace of the rows of a step, in bytes from its start.
 struct RowsLayout {
-  size_t q, row, ck, cv, ckexp, cvexp, total;
+  size_t q, row, ck, cv, cexp, total;
 };
 RowsLayout rows_layout(const dg_layer_desc& d, uint32_t n_seq, uint32_t MT, uint32_t n_ctiles) {
   const size_t heads = size_t(n_seq) * d.n_kv_heads, D = d.head_dim;
@@ -220,10 +214,8 @@ RowsLayout rows_layout(const dg_layer_desc& d, uint32_t n_seq, uint32_t MT, uint
   at = up(at + heads * n_ctiles * 2 * BLK * D);
   l.cv = at;
   at = up(at + heads * n_ctiles * 2 * BLK * D);
-  l.ckexp = at;
-  at = up(at + heads * n_ctiles * sizeof(int32_t));
-  l.cvexp = at;
-  at = up(at + heads * n_ctiles * sizeof(int32_t));
+  l.cexp = at;
+  at = up(at + heads * n_ctiles * 2 * sizeof(int32_t));
   l.total = at;
   return l;
 }
@@ -245,10 +237,14 @@ kv8::QueryParams query_params(const dg_layer_desc& d, uint8_t* ws, const RowsLay
 }
 
 // How many splits the key tiles of each sequence are cut into, so that the launch's CTAs end together: `per` tiles a CTA at
-// most, all CTAs of a wave side by side.  Costs in key tiles of a CTA.
-constexpr uint32_t kFixed8 = 6, kMerge8 = 4;
+// most, all CTAs of a wave side by side.  Costs in key tiles of a CTA (1.45 us): ten for what a wave costs beside its tiles; the
+// merge, 2 us and the partial rows' way through memory, 0.33 ns for each row and split.  One canvas of 256 rows, us: 32,768 keys
+// of 2 KV heads, splits 1 / 2 / 3 / 4 / 5 / 7 / 9: 396 / 216 / 158 / 125 / 194 / 160 / 150; window 1024 of 8 KV heads,
+// 1 / 2 / 3 / 4 / 6: 44 / 42 / 38 / 36 / 50; one token over 333 keys, 1 / 2 / 3: 26 / 21 / 19.
+constexpr uint32_t kFixed8 = 10;
 uint32_t plan_splits(const dg_ctx* c, kv8::AttnParams8& p, const uint32_t* cost, uint32_t* most_splits) {
   const uint32_t base = p.Hkv * p.MT * (p.D / 256u), sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u;
+  const uint64_t rows = uint64_t(p.n_seq) * p.C * p.Hq * (p.D / 256u);
   uint32_t most = 1;
   for (uint32_t b = 0; b < p.n_seq; ++b) most = cost[b] > most ? cost[b] : most;
   uint32_t best = most;
@@ -258,7 +254,7 @@ uint32_t plan_splits(const dg_ctx* c, kv8::AttnParams8& p, const uint32_t* cost,
     uint64_t ctas = 0;
     for (uint32_t b = 0; b < p.n_seq; ++b) ctas += uint64_t(base) * (cost[b] <= per ? 1u : (cost[b] + per - 1) / per);
     const uint64_t waves = (ctas + sms - 1) / sms;
-    const uint64_t t = waves * (per + kFixed8) * 16 + (S == 1 ? 0 : kMerge8 * 16 + S);
+    const uint64_t t = waves * (per + kFixed8) * 1000 + (S == 1 ? 0 : 1400 + rows * S * 23 / 100);
     if (t < best_cost) {
       best_cost = t;
       best = per;
@@ -327,8 +323,7 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
     cp.status = c->d_status;
     cp.k_codes = ws + l.ck;
     cp.v_codes = ws + l.cv;
-    cp.k_exp = reinterpret_cast<int32_t*>(ws + l.ckexp);
-    cp.v_exp = reinterpret_cast<int32_t*>(ws + l.cvexp);
+    cp.exps = reinterpret_cast<int32_t*>(ws + l.cexp);
     cp.n_ctiles = n_ctiles;
     kv8::AttnParams8 p = {};
     p.n_seq = n;
@@ -346,8 +341,7 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
     p.q_row = reinterpret_cast<const float2*>(ws + l.row);
     p.c_k = ws + l.ck;
     p.c_v = ws + l.cv;
-    p.c_kexp = cp.k_exp;
-    p.c_vexp = cp.v_exp;
+    p.c_exps = reinterpret_cast<const int2*>(cp.exps);
     p.n_ctiles = n_ctiles;
     p.out = static_cast<__nv_bfloat16*>(out) + b0 * q_elems;
     p.lse = lse ? lse + size_t(b0) * C * d->n_q_heads : nullptr;
@@ -359,8 +353,7 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
       kv8::Seq& s = p.seq[b];
       s.k = x->k;
       s.v = x->v;
-      s.k_exp = x->k_exp;
-      s.v_exp = x->v_exp;
+      s.exps = reinterpret_cast<const int2*>(x->exps);
       s.blocks = x->blocks;
       s.n_keys = n_keys[b0 + b];
       at[b] = pos ? pos[b0 + b] : s.n_keys;
@@ -411,7 +404,7 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   p.q_codes = qp.rows.codes;
   p.q_row = qp.rows.row;
   p.k = kv->k;
-  p.k_exp = kv->k_exp;
+  p.exps = reinterpret_cast<const int2*>(kv->exps);
   p.blocks = kv->blocks;
   p.n_keys = n_keys;
   p.C = C;
@@ -478,13 +471,11 @@ extern "C" int32_t dg_kv8_evict(dg_ctx* c, dg_kv8* from, uint32_t n_keys, const 
   p.ld_out = ld_out;
   p.k = from->k;
   p.v = from->v;
-  p.k_exp = from->k_exp;
-  p.v_exp = from->v_exp;
+  p.exps = from->exps;
   p.blocks = from->blocks;
   p.to_k = to->k;
   p.to_v = to->v;
-  p.to_kexp = to->k_exp;
-  p.to_vexp = to->v_exp;
+  p.to_exps = to->exps;
   p.to_blocks = to->blocks;
   c->last_launches = 2;
   DG_CUDA(kv8::launch_evict(p, c->stream));

@@ -21,16 +21,16 @@ namespace kv8 {
 
 constexpr uint32_t T_S = 0, T_O = 256;          // tensor memory: two S buffers of 128 columns, O
 constexpr float LAG = 3.0f, LIFT = 5.0f;        // 2^(LAG + LIFT) = 256 <= 448
-constexpr uint32_t SM_WARPS = 16, GROUP_WARPS = 8, W_K = 16, W_V = 17, W_MMA = 18, THREADS = 19 * 32;
-// B_P_FULL of a tile counts its eight softmax warps and the bytes of its first V unit; B_V2_FULL those of a canvas tile's second
-enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V2_FULL = 8, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 13, B_REF = 15, N_BARS = 17 };
+constexpr uint32_t SM_WARPS = 16, W_K = 16, W_V = 17, W_MMA = 18, THREADS = 19 * 32;
+// B_P_FULL of a tile counts its softmax warps and the bytes of its first V unit; B_V2_FULL those of a canvas tile's second
+enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V2_FULL = 8, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 13, N_BARS = 15 };
 
 template <uint32_t D> struct Cfg {
   static constexpr uint32_t KU = D / 256;                       // K units of a tile (32 KB each)
   static constexpr uint32_t NK = D == 256 ? 3 : 2, NV = D == 256 ? 2 : 1;   // stages
   static constexpr uint32_t Q_BYTES = 2 * BLK * D;
   static constexpr uint32_t O_K = Q_BYTES, O_V = O_K + NK * UNIT, O_X = O_V + NV * UNIT;
-  static constexpr uint32_t X_BYTES = (2 * 2 + 1) * BLK * 4;    // each group's row maxima (two threads a row); the reference
+  static constexpr uint32_t X_BYTES = 4 * BLK * 4;              // row maxima of a row's four threads
   static constexpr uint32_t O_BAR = O_X + X_BYTES, SMEM = O_BAR + N_BARS * 8 + 16;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
@@ -38,23 +38,19 @@ template <uint32_t D> struct Cfg {
 __device__ __forceinline__ void bar_sync_id(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-// 32 weights of a row from their scores: two words of e4m3 codes and two of e5m2 codes for every eight; sums into ls
+// 32 weights of a row from their scores: words of e4m3 codes and of e5m2 codes for every four; sums into ls
 __device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t c2, uint64_t sh2, uint64_t (&ls)[2], uint32_t (&p1)[8], uint32_t (&p2)[8]) {
 #pragma unroll
   for (uint32_t e = 0; e < 32; e += 4) {
-    uint16_t a[2], d[2];
+    float w[4];
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) {
-      float x0, x1;
-      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), c2, sh2), x0, x1);
-      const float q0 = fast_exp2(x0), q1 = fast_exp2(x1);
-      ls[j] = add_f32x2(ls[j], pack_f32x2(q0, q1));
-      const uint32_t h = pack_f16x2(q0, q1);
-      a[j] = e4m3x2_from_f16x2(h);
-      d[j] = e5m2x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(a[j])));
+      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), c2, sh2), w[2 * j], w[2 * j + 1]);
+      w[2 * j] = fast_exp2(w[2 * j]);
+      w[2 * j + 1] = fast_exp2(w[2 * j + 1]);
+      ls[j] = add_f32x2(ls[j], pack_f32x2(w[2 * j], w[2 * j + 1]));
     }
-    p1[e >> 2] = uint32_t(a[0]) | (uint32_t(a[1]) << 16);
-    p2[e >> 2] = uint32_t(d[0]) | (uint32_t(d[1]) << 16);
+    split4(w[0], w[1], w[2], w[3], &p1[e >> 2], &p2[e >> 2]);
   }
 }
 __device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
@@ -113,14 +109,14 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
   auto wait_unit = [&](uint32_t barrier, uint32_t stages, uint32_t n) -> bool {
     const uint32_t u = n < n_cached ? n : 2u * n + 1u - n_cached;
     bool ok = true;
-    if (n >= n_cached) ok = mbar_wait(bar(barrier + (u - 1u) % stages), ((u - 1u) / stages) & 1u, abort_flag);
-    return __all_sync(0xffffffffu, ok && mbar_wait(bar(barrier + u % stages), (u / stages) & 1u, abort_flag));
+    if (n >= n_cached) ok = bar_wait(bar(barrier + (u - 1u) % stages), ((u - 1u) / stages) & 1u, abort_flag);
+    return __all_sync(0xffffffffu, ok && bar_wait(bar(barrier + u % stages), (u / stages) & 1u, abort_flag));
   };
 
   if (tid == 0) {
     ctl[0] = 0u;
     for (uint32_t i = 0; i < N_BARS; ++i)
-      mbar_init(bar(i), i >= B_REF ? GROUP_WARPS : i >= B_P_FULL ? GROUP_WARPS + 1u : 1u);
+      mbar_init(bar(i), i >= B_P_FULL ? SM_WARPS + 1u : 1u);
     fence_mbar_init();
   }
   if (warp == W_MMA) {
@@ -135,114 +131,103 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
 
   const uint32_t head_tile = (b * p.Hkv + kvh) * p.n_ctiles;   // first canvas tile of this head
   float m_used = -INFINITY, l_run = 0.f;
-  // Softmax: two groups of eight warps take alternate tiles, so that one's latencies lie under the other's work; two threads
-  // a row, 64 score columns each.
-  const uint32_t quarter = warp & 3u, grp = (warp >> 3) & 1u, part = (warp >> 2) & 1u;
-  const uint32_t r = quarter * 32u + lane;                     // row
-  float* ref = xch + 4 * BLK;                                  // what the exponents of the last decided tile refer to
+  const uint32_t quarter = warp & 3u, part = warp >> 2;        // softmax: rows 32 quarter + lane, score columns 32 part ..
+  const uint32_t r = quarter * 32u + lane;
 
   if (warp < SM_WARPS) {
+    // What counts here is the time from a tile's scores to its weights: at most the 2,048 cycles of MMAs that are issued in
+    // between.  So all sixteen warps work on one tile, four threads a row (two groups of eight on alternate tiles: 1,640 cycles
+    // to the first half of P, 2,650 to the second).
     const uint32_t R = mt * BLK + r;
     const bool valid = R < rows_per_head;
     const RowVis rv = mask_row(mk, valid ? R / p.G : 0u);
     const float c_row = valid ? p.q_row[(size_t(b) * p.Hkv + kvh) * p.MT * BLK + R].x : 0.f;
     const bool warp_on = mt * BLK + quarter * 32u < rows_per_head;   // any row of this warp
-    const uint32_t t_s = tmem + ((quarter * 32u) << 16) + T_S + grp * 128u + part * 64u;
-    const uint32_t t_o = tmem + ((quarter * 32u) << 16) + T_O + part * 128u;
-    float* xm = xch + grp * 2u * BLK + r;
-    for (uint32_t n = grp; n < n_local; n += 2) {
-      const uint32_t t = n0 + n, ph = (n >> 1) & 1u;
-      const bool cached = t < ts.nA;
-      const uint32_t blk = cached ? ts.a0 + t : t - ts.nA;
-      int ek, ev;
-      if (cached) {
-        ek = sq.k_exp[size_t(kvh) * sq.blocks + blk];
-        ev = sq.v_exp[size_t(kvh) * sq.blocks + blk];
-      } else {
-        ek = p.c_kexp[head_tile + blk];
-        ev = p.c_vexp[head_tile + blk];
+    const uint32_t t_lane = tmem + ((quarter * 32u) << 16);
+    // what changes from tile to tile: the scales (requested a tile ahead), the first key, and at the first canvas tile the range
+    // of keys that the row sees
+    const int2* ep = sq.exps + size_t(kvh) * sq.blocks + ts.a0 + n0;
+    const int2* ec = p.c_exps + head_tile + (n0 > ts.nA ? n0 - ts.nA : 0u);
+    uint32_t lo = rv.lo, hi = mk.pre_hi, k0 = (ts.a0 + n0) * BLK + part * 32u, stage = 0, phase = 0;
+    int2 ex = make_int2(0, 0);
+    if (n_local > 0) ex = n_cached > 0 ? *ep : *ec;
+    if (n_cached == 0) ep = ec;
+    for (uint32_t n = 0; n < n_local; ++n) {
+      const uint32_t sb = n & 1u;
+      if (n == n_cached) {
+        lo = rv.can_lo;
+        hi = rv.can_hi;
+        k0 = mk.kv_len + (n0 > ts.nA ? n0 - ts.nA : 0u) * BLK + part * 32u;
       }
-      // head_dim 256: the scores are there when the tile's last K unit has been used
-      if (D == 256 ? !wait_unit(B_K_EMPTY, cf::NK, n) : !__all_sync(0xffffffffu, mbar_wait(bar(B_S_FULL + grp), ph, abort_flag))) break;
+      const int ek = ex.x, ev = ex.y;
+      ep = n + 1 == n_cached ? ec : ep + 1;
+      if (n + 1 < n_local) ex = *ep;
+      // head_dim 256: the scores are there when the tile's last K unit (a canvas tile's second) has been used
+      bool there;
+      if (D == 256) {
+        there = bar_wait(bar(B_K_EMPTY) + stage * 8u, phase, abort_flag);
+        if (++stage == cf::NK) { stage = 0; phase ^= 1u; }
+        if (n >= n_cached) {
+          there = there && bar_wait(bar(B_K_EMPTY) + stage * 8u, phase, abort_flag);
+          if (++stage == cf::NK) { stage = 0; phase ^= 1u; }
+        }
+      } else {
+        there = bar_wait(bar(B_S_FULL + sb), (n >> 1) & 1u, abort_flag);
+      }
+      if (!__all_sync(0xffffffffu, there)) break;
       if (!warp_on) {
         // rows behind the last one: their P stays whatever it is, no row of the output reads it
-        if (lane == 0) {
-          mbar_arrive(bar(B_REF + grp));
-          mbar_arrive(bar(B_P_FULL + grp));
-        }
+        if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
         continue;
       }
       tc_fence_after();
-      const uint32_t k0 = (cached ? blk * BLK : mk.kv_len + blk * BLK) + part * 64u;
-      const uint32_t lo = cached ? rv.lo : rv.can_lo, hi = cached ? mk.pre_hi : rv.can_hi;
       uint32_t s[32];
-      tmem_ld32(t_s, s);
+      tmem_ld32(t_lane + T_S + sb * 128u + part * 32u, s);
+      // the maxima of the tile before have been read by all: their warps have arrived
+      if (n != 0 && !__all_sync(0xffffffffu, bar_wait(bar(B_P_FULL + (sb ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
       tmem_wait_ld();
       hide32(s, lo, hi, k0);
+      k0 += BLK;
       float top = max32(s);
-      tmem_ld32(t_s + 32u, s);
-      tmem_wait_ld();
-      hide32(s, lo, hi, k0 + 32u);
-      top = fmaxf(top, max32(s));
-      xm[part * BLK] = top;
-      // the reference that the tile before was given
-      if (n != 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_REF + (grp ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
-      }
-      const float m_prev = n != 0 ? ref[r] : -INFINITY;
-      bar_sync_id(1u + grp * 4u + quarter, 64u);
-      top = fmaxf(top, xm[(part ^ 1u) * BLK]);
+      xch[part * BLK + r] = top;
       const float c = c_row * pow2i(ek);
+      // after this barrier all four threads of a row have their scores in registers: P may overwrite them
+      bar_sync_id(1u + quarter, 128u);
+      top = fmaxf(fmaxf(xch[r], xch[BLK + r]), fmaxf(xch[2 * BLK + r], xch[3 * BLK + r]));
       const float m_new = top * c + float(ev);
-      const bool need = n == 0 || m_new > m_prev + LAG;
-      const float m_ref = need ? m_new : m_prev;
-      if (part == 0) ref[r] = m_ref;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_REF + grp));
+      const bool need = n == 0 || m_new > m_used + LAG;
       if (n != 0 && __any_sync(0xffffffffu, need)) {
         // the outputs of the tile before: its last V unit has been used
         if (!wait_unit(B_V_EMPTY, cf::NV, n - 1u)) break;
         tc_fence_after();
-        const float alpha = need ? (m_prev == -INFINITY ? 0.f : fast_exp2(m_prev - m_new)) : 1.0f;
+        const float alpha = need ? (m_used == -INFINITY ? 0.f : fast_exp2(m_used - m_new)) : 1.0f;
 #pragma unroll 1
-        for (uint32_t cc = 0; cc < 4; ++cc) {
+        for (uint32_t cc = 0; cc < 2; ++cc) {
           uint32_t o[32];
-          tmem_ld32(t_o + cc * 32u, o);
+          tmem_ld32(t_lane + T_O + part * 64u + cc * 32u, o);
           tmem_wait_ld();
 #pragma unroll
           for (uint32_t e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(t_o + cc * 32u, o);
+          tmem_st32(t_lane + T_O + part * 64u + cc * 32u, o);
         }
+        l_run *= alpha;
       }
-      // this thread's sum may stand at an older reference
-      if (m_ref != m_used) {
-        l_run = m_used == -INFINITY ? 0.f : l_run * fast_exp2(m_used - m_ref);
-        m_used = m_ref;
-      }
-      const float shift = (m_ref == -INFINITY ? 0.f : -m_ref) + float(ev) + LIFT;
+      if (need) m_used = m_new;
+      const float shift = (m_used == -INFINITY ? 0.f : -m_used) + float(ev) + LIFT;
       const uint64_t c2 = pack_f32x2(c, c), sh2 = pack_f32x2(shift, shift);
       uint64_t ls[2] = {0ull, 0ull};
-      // P goes over the second half of the thread's own score columns, which it has in registers: 8 columns each of p1 of
-      // the first and second 32 keys, then p2
       uint32_t p1[8], p2[8];
       weights32(s, c2, sh2, ls, p1, p2);
-      tmem_st8(t_s + 40u, p1);
-      tmem_st8(t_s + 56u, p2);
-      tmem_ld32(t_s, s);
-      tmem_wait_ld();
-      hide32(s, lo, hi, k0);
-      weights32(s, c2, sh2, ls, p1, p2);
-      tmem_st8(t_s + 32u, p1);
-      tmem_st8(t_s + 48u, p2);
-      {
-        float a, d;
-        unpack_f32x2(add_f32x2(ls[0], ls[1]), a, d);
-        l_run = fmaf(a + d, pow2i(-ev), l_run);
-      }
+      // the 32 keys of a thread are the K of one MMA: columns 8 part .. of p1, of p2 32 columns on
+      tmem_st8(t_lane + T_S + sb * 128u + part * 8u, p1);
+      tmem_st8(t_lane + T_S + sb * 128u + 32u + part * 8u, p2);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_P_FULL + grp));
+      if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+      float a, d;
+      unpack_f32x2(add_f32x2(ls[0], ls[1]), a, d);
+      l_run = fmaf(a + d, pow2i(-ev), l_run);
     }
   } else if (warp == W_K) {
     if (lane == 0 && n_local > 0) {
@@ -258,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
         const uint32_t units = cached ? cf::KU : 2 * cf::KU;
         for (uint32_t i = 0; i < units; ++i, ++u) {
           const uint32_t st = u % cf::NK;
-          if (u >= cf::NK && !mbar_wait(bar(B_K_EMPTY + st), (u / cf::NK - 1u) & 1u, abort_flag)) { ok = false; break; }
+          if (u >= cf::NK && !bar_wait(bar(B_K_EMPTY + st), (u / cf::NK - 1u) & 1u, abort_flag)) { ok = false; break; }
           mbar_expect_tx(bar(B_K_FULL + st), UNIT);
           bulk_load(s0 + cf::O_K + st * UNIT, src + size_t(i) * UNIT, UNIT, bar(B_K_FULL + st));
         }
@@ -274,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
                                      : p.c_v + size_t(head_tile + t - ts.nA) * 2u * BLK * D) + size_t(z) * UNIT;
         for (uint32_t i = 0; i < (cached ? 1u : 2u); ++i, ++u) {
           const uint32_t st = u % cf::NV;
-          if (u >= cf::NV && !mbar_wait(bar(B_V_EMPTY + st), (u / cf::NV - 1u) & 1u, abort_flag)) { ok = false; break; }
+          if (u >= cf::NV && !bar_wait(bar(B_V_EMPTY + st), (u / cf::NV - 1u) & 1u, abort_flag)) { ok = false; break; }
           const uint32_t full = bar(i == 0 ? B_P_FULL + ((t - n0) & 1u) : B_V2_FULL);
           mbar_expect_tx(full, UNIT);
           bulk_load(s0 + cf::O_V + st * UNIT, src + size_t(i) * BLK * D, UNIT, full);
@@ -292,14 +277,14 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     constexpr uint32_t IDESC = idesc_f8(128, 128, 0, 0), IDESC_P1 = idesc_f8(128, 256, 0, 1), IDESC_P2 = idesc_f8(128, 256, 1, 1);
     const uint32_t dq = ((s0 >> 4) & 0x3fffu) | (1u << 16), dk = (((s0 + cf::O_K) >> 4) & 0x3fffu) | (1u << 16);
     const uint32_t dv = (((s0 + cf::O_V) >> 4) & 0x3fffu) | ((SLAB >> 4) << 16);   // MN-major: 128-column chunks SLAB apart
-    bool ok = __all_sync(0xffffffffu, mbar_wait(bar(B_Q), 0u, abort_flag));
+    bool ok = __all_sync(0xffffffffu, bar_wait(bar(B_Q), 0u, abort_flag));
     uint32_t uk = 0, uv = 0;
     auto issue_qk = [&](uint32_t n) -> bool {
       const uint32_t units = n < n_cached ? cf::KU : 2 * cf::KU;
       const uint32_t d_tmem = tmem + T_S + (n & 1u) * 128u;
       for (uint32_t i = 0; i < units; ++i, ++uk) {
         const uint32_t st = uk % cf::NK;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_K_FULL + st), (uk / cf::NK) & 1u, abort_flag))) return false;
+        if (!__all_sync(0xffffffffu, bar_wait(bar(B_K_FULL + st), (uk / cf::NK) & 1u, abort_flag))) return false;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t qa = dq + (((i % cf::KU) * UNIT) >> 4), kb = dk + st * (UNIT >> 4);
@@ -324,8 +309,8 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       const uint32_t keys = n < n_cached ? BLK : p.C - (n0 + n - ts.nA) * BLK;
       const uint32_t pt = tmem + T_S + (n & 1u) * 128u;
       for (uint32_t i = 0; i < units; ++i, ++uv) {
-        ok = __all_sync(0xffffffffu, i == 0 ? mbar_wait(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag)
-                                            : mbar_wait(bar(B_V2_FULL), (n - n_cached) & 1u, abort_flag));
+        ok = __all_sync(0xffffffffu, i == 0 ? bar_wait(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag)
+                                            : bar_wait(bar(B_V2_FULL), (n - n_cached) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -333,9 +318,8 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
 #pragma unroll
           for (uint32_t ks = 0; ks < 4; ++ks) {
             if (ks != 0 && ks * 32u >= keys) break;
-            const uint32_t a = pt + (ks >> 1) * 64u + 32u + (ks & 1u) * 8u;
-            mma_ts(tmem + T_O, a, desc(vb + ks * (4096u >> 4)), IDESC_P1, ks == 0 ? (n | i) != 0u : 1u);
-            mma_ts(tmem + T_O, a + 16u, desc(vb + ks * (4096u >> 4)), IDESC_P2, 1u);
+            mma_ts(tmem + T_O, pt + ks * 8u, desc(vb + ks * (4096u >> 4)), IDESC_P1, ks == 0 ? (n | i) != 0u : 1u);
+            mma_ts(tmem + T_O, pt + 32u + ks * 8u, desc(vb + ks * (4096u >> 4)), IDESC_P2, 1u);
           }
           umma_commit(bar(B_V_EMPTY + st));
           if (n + 1 == n_local && i + 1 == units) umma_commit(bar(B_O));
@@ -349,18 +333,14 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
   if (warp < SM_WARPS) {
     bool have = __all_sync(0xffffffffu, n_local > 0 && !*abort_flag);
     if (have) {
-      have = __all_sync(0xffffffffu, mbar_wait(bar(B_O), 0u, abort_flag));
+      have = __all_sync(0xffffffffu, bar_wait(bar(B_O), 0u, abort_flag));
       tc_fence_after();
     }
-    // the row's sum is its four threads' sums, at the last reference
-    float* xl = xch;
-    const bool any = n_local > 0 && mt * BLK + quarter * 32u < rows_per_head;
-    bar_sync_id(9u + quarter, 128u);
-    const float m_row = any ? ref[r] : -INFINITY;
-    l_run = m_row == m_used ? l_run : (m_used == -INFINITY ? 0.f : l_run * fast_exp2(m_used - m_row));
-    xl[(grp * 2u + part) * BLK + r] = l_run;
-    bar_sync_id(9u + quarter, 128u);
-    const float l = (xl[r] + xl[BLK + r]) + (xl[2 * BLK + r] + xl[3 * BLK + r]);
+    // the row's sum is its four threads' sums
+    bar_sync_id(1u + quarter, 128u);
+    xch[part * BLK + r] = l_run;
+    bar_sync_id(1u + quarter, 128u);
+    const float l = (xch[r] + xch[BLK + r]) + (xch[2 * BLK + r] + xch[3 * BLK + r]);
     const bool direct = sq.n_splits == 1;
     const float mul = direct ? (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) : 1.0f;   // a sum that is NaN stays one
     const uint32_t t_lane = tmem + ((quarter * 32u) << 16);
@@ -378,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     }
 #pragma unroll 1
     for (uint32_t cc = 0; cc < 2; ++cc) {
-      const uint32_t col = (grp * 2u + part) * 64u + cc * 32u;
+      const uint32_t col = part * 64u + cc * 32u;
       uint32_t o[32];
       if (have) {
         tmem_ld32(t_lane + T_O + col, o);
@@ -406,12 +386,12 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       __syncwarp();
     }
     const uint32_t R = mt * BLK + r;
-    if (part == 0 && grp == 0 && R < rows_per_head) {
+    if (part == 0 && R < rows_per_head) {
       if (!direct)
-        p.ws_ml[size_t(blockIdx.x) * BLK + r] = make_float2(m_row, l);
+        p.ws_ml[size_t(blockIdx.x) * BLK + r] = make_float2(m_used, l);
       else if (p.lse != nullptr && z == 0)
         p.lse[(size_t(b) * p.C + R / p.G) * p.Hq + kvh * p.G + R % p.G] =
-            l == 0.f ? -INFINITY : (m_row - LIFT + log2f(l)) * 0.6931471805599453f;
+            l == 0.f ? -INFINITY : (m_used - LIFT + log2f(l)) * 0.6931471805599453f;
     }
   }
 

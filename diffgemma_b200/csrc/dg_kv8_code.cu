@@ -221,7 +221,7 @@ __device__ __forceinline__ void store_canvas_row(const CodeParams& p, bool is_k,
       *reinterpret_cast<uint2*>(dst + BLK * D + off) = rest;
     }
   }
-  if (lane == 0 && r == 0) (is_k ? p.k_exp : p.v_exp)[tile] = e;
+  if (lane == 0 && r == 0) p.exps[tile * 2 + (is_k ? 0 : 1)] = e;
 }
 
 template <int NJ>
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(CT, 2) dg_kv8_append_kernel(const __grid_const
   const uint32_t kept = p.n_keys > t0 ? p.n_keys - t0 : 0u;
   const uint32_t n_rows = end - t0 < BLK ? end - t0 : BLK;
   uint8_t* codes = (is_k ? p.k_codes : p.v_codes) + (size_t(h) * p.blocks + blk) * BLK * D;
-  int32_t* exps = (is_k ? p.k_exp : p.v_exp) + size_t(h) * p.blocks + blk;
+  int32_t* exps = p.exps + (size_t(h) * p.blocks + blk) * 2 + (is_k ? 0 : 1);
   const __nv_bfloat16* src = is_k ? p.k : p.v;
   // row s of this warp
   auto row = [&](uint32_t s) { return rank * TOK + (s >> 1) * APASS + warp * 2u + (s & 1u); };
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(256) dg_kv8_read_kernel(const __grid_constant_
     const uint32_t h = uint32_t(row % p.Hkv), slot = p.slot0 + uint32_t(row / p.Hkv);
     const size_t blk = size_t(h) * p.blocks + slot / BLK;
     const uint8_t* src = (is_k ? p.k : p.v) + blk * BLK * p.D + (c >> 3) * SLAB + chunk_off(slot % BLK, c & 7u);
-    const float mul = pow2i((is_k ? p.k_exp : p.v_exp)[blk]);
+    const float mul = pow2i(p.exps[blk * 2 + (is_k ? 0 : 1)]);
     const uint4 v = *reinterpret_cast<const uint4*>(src);
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[8];

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(512) dg_kv8_move_kernel(const __grid_constant_
   const uint32_t rows = p.n_keep - blk * BLK < BLK ? p.n_keep - blk * BLK : BLK;
   const int32_t* kept = p.kept + size_t(h) * p.n_keep + blk * BLK;
   const uint8_t* src = (is_k ? p.k : p.v) + size_t(h) * p.blocks * BLK * D;
-  const int32_t* from = (is_k ? p.k_exp : p.v_exp) + size_t(h) * p.blocks;
+  const int32_t* from = p.exps + size_t(h) * p.blocks * 2 + (is_k ? 0 : 1);
   uint4 v[PER];
   float top = 0.f;
 #pragma unroll
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(512) dg_kv8_move_kernel(const __grid_constant_
     if (r < rows) {
       const uint32_t slot = uint32_t(kept[r]);
       v[i] = *reinterpret_cast<const uint4*>(src + size_t(slot / BLK) * BLK * D + (c >> 3) * SLAB + chunk_off(slot % BLK, c & 7u));
-      const int e = from[slot / BLK];
+      const int e = from[slot / BLK * 2];
       if (c == 0) exps[r] = e;
       uint32_t m = __vmaxu4(__vmaxu4(v[i].x & 0x7f7f7f7fu, v[i].y & 0x7f7f7f7fu), __vmaxu4(v[i].z & 0x7f7f7f7fu, v[i].w & 0x7f7f7f7fu));
       m = __vmaxu4(m, m >> 16);
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(512) dg_kv8_move_kernel(const __grid_constant_
     }
     *reinterpret_cast<uint4*>(dst + (c >> 3) * SLAB + chunk_off(r, c & 7u)) = v[i];
   }
-  if (tid == 0) (is_k ? p.to_kexp : p.to_vexp)[size_t(h) * p.to_blocks + blk] = e;
+  if (tid == 0) p.to_exps[(size_t(h) * p.to_blocks + blk) * 2 + (is_k ? 0 : 1)] = e;
 }
 
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st) {

@@ -72,13 +72,13 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
     const uint32_t kt = g * cf::COLS / cf::NR, col0 = g * cf::COLS % cf::NR;
     const uint32_t key = quarter * 32u + lane, t = (first + kt) * BLK + key;
     const bool live = t < p.n_keys;
-    const float kscale = kt < have ? pow2i(p.k_exp[size_t(kvh) * p.blocks + first + kt]) : 0.f;
+    const float kscale = kt < have ? pow2i(p.exps[size_t(kvh) * p.blocks + first + kt].x) : 0.f;
     // keys that some row does not see: a look at each row's window
     const bool edge = (first + kt) * BLK < mask_row_lo(mk, p.C - 1);
     float acc[2] = {0.f, 0.f};
     for (uint32_t n = 0; n < n_steps; ++n) {
       const uint32_t sb = n & 1u;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(WB_S_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
+      if (!__all_sync(0xffffffffu, bar_wait(bar(WB_S_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
       tc_fence_after();
       const float4* cst = reinterpret_cast<const float4*>(smem + cf::O_C + ((n & 3u) * cf::NR + col0) * 8u);
       const uint32_t src = tmem + ((quarter * 32u) << 16) + sb * (cf::KT * cf::NR) + kt * cf::NR + col0;
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
       for (uint32_t o = 0; o < have * BLK * D; o += UNIT) bulk_load(s0 + o, k + o, UNIT, bar(WB_K));
       for (uint32_t n = 0; n < n_steps; ++n) {
         const uint32_t sb = n & 1u, full = bar(WB_Q_FULL + sb), step = st0 + n;
-        if (n > 1 && !mbar_wait(bar(WB_Q_EMPTY + sb), ((n - 2) >> 1) & 1u, abort_flag)) break;
+        if (n > 1 && !bar_wait(bar(WB_Q_EMPTY + sb), ((n - 2) >> 1) & 1u, abort_flag)) break;
         // the constants' slot was last read for step n - 4, which S^T of step n - 2 waited for
         mbar_expect_tx(full, cf::STAGE + cf::NR * 8u);
         const uint32_t dst = s0 + cf::O_Q + sb * cf::STAGE;
@@ -151,11 +151,11 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
   } else if (n_steps > 0) {
     constexpr uint32_t IDESC = idesc_f8(128, cf::NR, 0, 0);
     const uint64_t dk = umma_smem_desc(s0, 16, 1024), dq = umma_smem_desc(s0 + cf::O_Q, 16, 1024);
-    bool ok = __all_sync(0xffffffffu, mbar_wait(bar(WB_K), 0u, abort_flag));
+    bool ok = __all_sync(0xffffffffu, bar_wait(bar(WB_K), 0u, abort_flag));
     for (uint32_t n = 0; ok && n < n_steps; ++n) {
       const uint32_t sb = n & 1u;
-      if (n > 1 && !__all_sync(0xffffffffu, mbar_wait(bar(WB_S_EMPTY + sb), ((n - 2) >> 1) & 1u, abort_flag))) break;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(WB_Q_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
+      if (n > 1 && !__all_sync(0xffffffffu, bar_wait(bar(WB_S_EMPTY + sb), ((n - 2) >> 1) & 1u, abort_flag))) break;
+      if (!__all_sync(0xffffffffu, bar_wait(bar(WB_Q_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll 1
