@@ -24,9 +24,10 @@ constexpr uint32_t BLK = 128;                  // tokens of a block
 constexpr uint32_t SLAB = BLK * 128;           // bytes of a slab: 128 tokens x 128 dims
 constexpr uint32_t UNIT = 2 * SLAB;            // what one bulk copy brings: 128 tokens x 256 dims
 constexpr int EXP_MIN = -60, EXP_MAX = 60;     // sums of scales of one row stay inside fp32
+constexpr float LIFT = 5.0f;                   // partial rows: weights stand at 2^LIFT times their reference
 constexpr uint32_t MAX_SEQ = 64;               // caches served by one launch
 
-enum : uint32_t { KID_CODE = 16, KID_ATTN = 17, KID_WEIGHTS = 18, KID_EVICT = 19 };
+enum : uint32_t { KID_CODE = 16, KID_ATTN = 17, KID_WEIGHTS = 18, KID_EVICT = 19, KID_TOKEN = 20 };
 
 // byte offset of 16-byte chunk c (of 8 per slab) of token r in a slab
 __host__ __device__ __forceinline__ uint32_t chunk_off(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
@@ -52,6 +53,11 @@ __device__ __forceinline__ int scale_exp(float top) {
 __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2_from_e5m2x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(r) : "h"(v));
   return r;
 }
 __device__ __forceinline__ uint32_t f16x2_from_e4m3x2(uint16_t v) {
@@ -85,6 +91,21 @@ __device__ __forceinline__ void split4(float a, float b, float c, float d, uint3
   *p1 = e4m3x4_half(a, b, c, d);
   const uint32_t lo = f16x2_from_e4m3x2(uint16_t(*p1)), hi = f16x2_from_e4m3x2(uint16_t(*p1 >> 16));
   *p2 = e5m2x4_half(sub_f32_f16(a, uint16_t(lo)), sub_f32_f16(b, uint16_t(lo >> 16)), sub_f32_f16(c, uint16_t(hi)), sub_f32_f16(d, uint16_t(hi >> 16)));
+}
+
+// Four weights as three e5m2 terms: within 2^-9 of a weight down to 2^-12, within 2^-17 below
+__device__ __forceinline__ void split4_e5m2(float a, float b, float c, float d, uint32_t (&t)[3]) {
+  float x[4] = {a, b, c, d};
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    t[i] = e5m2x4_half(x[0], x[1], x[2], x[3]);
+    if (i == 2) break;
+    const uint32_t lo = f16x2_from_e5m2x2(uint16_t(t[i])), hi = f16x2_from_e5m2x2(uint16_t(t[i] >> 16));
+    x[0] = sub_f32_f16(x[0], uint16_t(lo));
+    x[1] = sub_f32_f16(x[1], uint16_t(lo >> 16));
+    x[2] = sub_f32_f16(x[2], uint16_t(hi));
+    x[3] = sub_f32_f16(x[3], uint16_t(hi >> 16));
+  }
 }
 
 // ---- tensor cores: kind::f8f6f4, fp32 accumulate.  A e4m3 (0) or e5m2 (1), B e4m3; other fields as for bf16.
@@ -213,6 +234,28 @@ struct AttnParams8 {
   DevStatus* status;
 };
 
+// few query rows: the queries, and up to TOKEN_CANVAS canvas keys, raw
+constexpr uint32_t TOKEN_ROWS = 16, TOKEN_CANVAS = 8;
+struct TokenParams {
+  Seq seq[MAX_SEQ];
+  uint64_t pos[MAX_SEQ];
+  uint32_t n_seq, C, Hq, Hkv, G, D;
+  uint32_t mode, windowed, wm1, v_norm;
+  const __nv_bfloat16* q;      // [seq][C][Hq][D]
+  const __nv_bfloat16* k;      // [seq][C][Hkv][D], or null: the cached keys alone
+  const __nv_bfloat16* v;
+  const __nv_bfloat16* qw;
+  const __nv_bfloat16* kw;
+  __nv_bfloat16* q_rot;
+  __nv_bfloat16* out;
+  float* lse;
+  float* ws_o;                 // split partials [CTA][D / 256][128][256]
+  float2* ws_ml;
+  DevStatus* status;
+  float eps, scale_log2;
+  Rope rope;
+};
+
 struct WeightParams {
   const uint8_t* q_codes;
   const float2* q_row;
@@ -294,6 +337,8 @@ cudaError_t configure();
 cudaError_t launch_rows(const QueryParams& q, const CodeParams& p, const uint64_t* pos, uint32_t n_seq, cudaStream_t st);
 cudaError_t launch_append(const CodeParams& p, cudaStream_t st);
 cudaError_t launch_read(const ReadParams& p, cudaStream_t st);
+cudaError_t launch_token(const TokenParams& p, uint32_t D, uint32_t n_ctas, cudaStream_t st);
+cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_t st);
 cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st);
 cudaError_t launch_weights(const WeightParams& p, uint32_t D, cudaStream_t st);
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st);

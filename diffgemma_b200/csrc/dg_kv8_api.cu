@@ -11,10 +11,12 @@ namespace kv8 {
 cudaError_t configure_code();
 cudaError_t configure_attn();
 cudaError_t configure_weights();
+cudaError_t configure_token();
 cudaError_t configure() {
   cudaError_t e = configure_code();
   if (e == cudaSuccess) e = configure_attn();
   if (e == cudaSuccess) e = configure_weights();
+  if (e == cudaSuccess) e = configure_token();
   return e;
 }
 }  // namespace kv8
@@ -241,20 +243,21 @@ kv8::QueryParams query_params(const dg_layer_desc& d, uint8_t* ws, const RowsLay
 // merge, 2 us and the partial rows' way through memory, 0.33 ns for each row and split.  One canvas of 256 rows, us: 32,768 keys
 // of 2 KV heads, splits 1 / 2 / 3 / 4 / 5 / 7 / 9: 396 / 216 / 158 / 125 / 194 / 160 / 150; window 1024 of 8 KV heads,
 // 1 / 2 / 3 / 4 / 6: 44 / 42 / 38 / 36 / 50; one token over 333 keys, 1 / 2 / 3: 26 / 21 / 19.
-constexpr uint32_t kFixed8 = 10;
-uint32_t plan_splits(const dg_ctx* c, kv8::AttnParams8& p, const uint32_t* cost, uint32_t* most_splits) {
-  const uint32_t base = p.Hkv * p.MT * (p.D / 256u), sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u;
-  const uint64_t rows = uint64_t(p.n_seq) * p.C * p.Hq * (p.D / 256u);
+// Single tokens (dg_kv8_token_kernel), all dims in one CTA: what a wave costs beside its tiles is TOKEN_FIXED.
+constexpr uint32_t kFixed8 = 10, kFixedToken = 6;
+uint32_t plan_splits(const dg_ctx* c, kv8::Seq* seq, uint32_t n_seq, uint32_t base, uint64_t rows, uint32_t fixed, const uint32_t* cost,
+                     uint32_t* most_splits) {
+  const uint32_t sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u;
   uint32_t most = 1;
-  for (uint32_t b = 0; b < p.n_seq; ++b) most = cost[b] > most ? cost[b] : most;
+  for (uint32_t b = 0; b < n_seq; ++b) most = cost[b] > most ? cost[b] : most;
   uint32_t best = most;
   uint64_t best_cost = ~0ull;
   for (uint32_t S = 1; S <= 128 && S <= most; ++S) {
     const uint32_t per = (most + S - 1) / S;
     uint64_t ctas = 0;
-    for (uint32_t b = 0; b < p.n_seq; ++b) ctas += uint64_t(base) * (cost[b] <= per ? 1u : (cost[b] + per - 1) / per);
+    for (uint32_t b = 0; b < n_seq; ++b) ctas += uint64_t(base) * (cost[b] <= per ? 1u : (cost[b] + per - 1) / per);
     const uint64_t waves = (ctas + sms - 1) / sms;
-    const uint64_t t = waves * (per + kFixed8) * 1000 + (S == 1 ? 0 : 1400 + rows * S * 23 / 100);
+    const uint64_t t = waves * (per + fixed) * 1000 + (S == 1 ? 0 : 1400 + rows * S * 23 / 100);
     if (t < best_cost) {
       best_cost = t;
       best = per;
@@ -262,11 +265,11 @@ uint32_t plan_splits(const dg_ctx* c, kv8::AttnParams8& p, const uint32_t* cost,
   }
   uint32_t ctas = 0;
   *most_splits = 1;
-  for (uint32_t b = 0; b < p.n_seq; ++b) {
+  for (uint32_t b = 0; b < n_seq; ++b) {
     uint32_t s = cost[b] <= best ? 1u : (cost[b] + best - 1) / best;
     if (c->forced_splits) s = c->forced_splits < cost[b] ? c->forced_splits : (cost[b] ? cost[b] : 1u);
-    p.seq[b].first_cta = ctas;
-    p.seq[b].n_splits = s;
+    seq[b].first_cta = ctas;
+    seq[b].n_splits = s;
     ctas += base * s;
     *most_splits = s > *most_splits ? s : *most_splits;
   }
@@ -297,34 +300,12 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
   if (r != DG_OK) return r;
   DG_CUDA(cudaSetDevice(c->device));
   const uint32_t C = d->canvas, G = d->n_q_heads / d->n_kv_heads, D = d->head_dim;
-  const uint32_t MT = (C * G + BLK - 1) / BLK, n_ctiles = k ? (C + BLK - 1) / BLK : 0;
+  const uint32_t MT = (C * G + BLK - 1) / BLK, n_ctiles = k ? (C + BLK - 1) / BLK : 0, KU = D / 256;
+  const bool token = C * G <= kv8::TOKEN_ROWS && C <= kv8::TOKEN_CANVAS;
   const size_t q_elems = size_t(C) * d->n_q_heads * D, kv_elems = size_t(C) * d->n_kv_heads * D;
   c->last_launches = 0;
   for (uint32_t b0 = 0; b0 < batch; b0 += kv8::MAX_SEQ) {
     const uint32_t n = batch - b0 < kv8::MAX_SEQ ? batch - b0 : kv8::MAX_SEQ;
-    const RowsLayout l = rows_layout(*d, n, MT, n_ctiles);
-    r = grow_bytes(c, &c->kv8_rows, &c->kv8_rows_bytes, l.total);
-    if (r != DG_OK) return r;
-    uint8_t* ws = c->kv8_rows;
-    kv8::QueryParams qp = query_params(*d, ws, l, MT);
-    qp.q = static_cast<const __nv_bfloat16*>(q) + b0 * q_elems;
-    qp.qw = static_cast<const __nv_bfloat16*>(qw);
-    qp.q_rot = q_rot ? static_cast<__nv_bfloat16*>(q_rot) + b0 * q_elems : nullptr;
-    kv8::CodeParams cp = {};
-    cp.k = k ? static_cast<const __nv_bfloat16*>(k) + b0 * kv_elems : nullptr;
-    cp.v = v ? static_cast<const __nv_bfloat16*>(v) + b0 * kv_elems : nullptr;
-    cp.kw = static_cast<const __nv_bfloat16*>(kw);
-    cp.n = C;
-    cp.Hkv = d->n_kv_heads;
-    cp.D = D;
-    cp.v_norm = d->v_norm;
-    cp.eps = d->rms_eps;
-    cp.rope = qp.rope;
-    cp.status = c->d_status;
-    cp.k_codes = ws + l.ck;
-    cp.v_codes = ws + l.cv;
-    cp.exps = reinterpret_cast<int32_t*>(ws + l.cexp);
-    cp.n_ctiles = n_ctiles;
     kv8::AttnParams8 p = {};
     p.n_seq = n;
     p.C = C;
@@ -337,11 +318,6 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
     p.mode = d->mask_mode;
     p.windowed = windowed ? 1u : 0u;
     p.wm1 = windowed ? d->window - 1u : 0u;
-    p.q_codes = ws + l.q;
-    p.q_row = reinterpret_cast<const float2*>(ws + l.row);
-    p.c_k = ws + l.ck;
-    p.c_v = ws + l.cv;
-    p.c_exps = reinterpret_cast<const int2*>(cp.exps);
     p.n_ctiles = n_ctiles;
     p.out = static_cast<__nv_bfloat16*>(out) + b0 * q_elems;
     p.lse = lse ? lse + size_t(b0) * C * d->n_q_heads : nullptr;
@@ -357,17 +333,87 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
       s.blocks = x->blocks;
       s.n_keys = n_keys[b0 + b];
       at[b] = pos ? pos[b0 + b] : s.n_keys;
-      cost[b] = kv8::tile_cost(kv8::tiles_of(kv8::seq_mask(p, s.n_keys), 0, C - 1));
+      const kv8::Tiles t = kv8::tiles_of(kv8::seq_mask(p, s.n_keys), 0, C - 1);
+      cost[b] = token ? t.nA : kv8::tile_cost(t);
     }
     uint32_t splits = 1;
-    const uint32_t ctas = plan_splits(c, p, cost, &splits);
+    const uint64_t rows = uint64_t(n) * C * d->n_q_heads * KU;
+    const uint32_t ctas = plan_splits(c, p.seq, n, token ? p.Hkv : p.Hkv * MT * KU, rows, token ? kFixedToken : kFixed8, cost, &splits);
     if (splits > 1) {
-      const size_t rows = size_t(ctas) * BLK;
-      r = grow_bytes(c, &c->kv8_part, &c->kv8_part_bytes, rows * (256 * sizeof(float) + sizeof(float2)));
+      const size_t slots = size_t(ctas) * (token ? KU : 1u) * BLK;
+      r = grow_bytes(c, &c->kv8_part, &c->kv8_part_bytes, slots * (256 * sizeof(float) + sizeof(float2)));
       if (r != DG_OK) return r;
       p.ws_o = reinterpret_cast<float*>(c->kv8_part);
-      p.ws_ml = reinterpret_cast<float2*>(c->kv8_part + rows * 256 * sizeof(float));
+      p.ws_ml = reinterpret_cast<float2*>(c->kv8_part + slots * 256 * sizeof(float));
     }
+    const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q) + b0 * q_elems;
+    const __nv_bfloat16* kb = k ? static_cast<const __nv_bfloat16*>(k) + b0 * kv_elems : nullptr;
+    const __nv_bfloat16* vb = v ? static_cast<const __nv_bfloat16*>(v) + b0 * kv_elems : nullptr;
+    __nv_bfloat16* rot = q_rot ? static_cast<__nv_bfloat16*>(q_rot) + b0 * q_elems : nullptr;
+    if (token) {
+      kv8::TokenParams t = {};
+      for (uint32_t b = 0; b < n; ++b) {
+        t.seq[b] = p.seq[b];
+        t.pos[b] = at[b];
+        p.seq[b].first_cta *= KU;                 // the merge counts in 256 columns
+      }
+      t.n_seq = n;
+      t.C = C;
+      t.Hq = p.Hq;
+      t.Hkv = p.Hkv;
+      t.G = G;
+      t.D = D;
+      t.mode = p.mode;
+      t.windowed = p.windowed;
+      t.wm1 = p.wm1;
+      t.v_norm = d->v_norm;
+      t.q = qb;
+      t.k = kb;
+      t.v = vb;
+      t.qw = static_cast<const __nv_bfloat16*>(qw);
+      t.kw = static_cast<const __nv_bfloat16*>(kw);
+      t.q_rot = rot;
+      t.out = p.out;
+      t.lse = p.lse;
+      t.ws_o = p.ws_o;
+      t.ws_ml = p.ws_ml;
+      t.status = c->d_status;
+      t.eps = d->rms_eps;
+      t.scale_log2 = d->softmax_scale * 1.4426950408889634f;
+      t.rope = make_rope8(*d);
+      DG_CUDA(kv8::launch_token(t, D, ctas, c->stream));
+      if (splits > 1) DG_CUDA(kv8::launch_merge(p, splits, c->stream));
+      c->last_launches += splits > 1 ? 2 : 1;
+      continue;
+    }
+    const RowsLayout l = rows_layout(*d, n, MT, n_ctiles);
+    r = grow_bytes(c, &c->kv8_rows, &c->kv8_rows_bytes, l.total);
+    if (r != DG_OK) return r;
+    uint8_t* ws = c->kv8_rows;
+    kv8::QueryParams qp = query_params(*d, ws, l, MT);
+    qp.q = qb;
+    qp.qw = static_cast<const __nv_bfloat16*>(qw);
+    qp.q_rot = rot;
+    kv8::CodeParams cp = {};
+    cp.k = kb;
+    cp.v = vb;
+    cp.kw = static_cast<const __nv_bfloat16*>(kw);
+    cp.n = C;
+    cp.Hkv = d->n_kv_heads;
+    cp.D = D;
+    cp.v_norm = d->v_norm;
+    cp.eps = d->rms_eps;
+    cp.rope = qp.rope;
+    cp.status = c->d_status;
+    cp.k_codes = ws + l.ck;
+    cp.v_codes = ws + l.cv;
+    cp.exps = reinterpret_cast<int32_t*>(ws + l.cexp);
+    cp.n_ctiles = n_ctiles;
+    p.q_codes = ws + l.q;
+    p.q_row = reinterpret_cast<const float2*>(ws + l.row);
+    p.c_k = ws + l.ck;
+    p.c_v = ws + l.cv;
+    p.c_exps = reinterpret_cast<const int2*>(cp.exps);
     DG_CUDA(kv8::launch_rows(qp, cp, at, n, c->stream));
     DG_CUDA(kv8::launch_attention(p, ctas, splits, c->stream));
     c->last_launches += splits > 1 ? 3 : 2;

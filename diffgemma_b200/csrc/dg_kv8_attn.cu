@@ -20,7 +20,7 @@ namespace dg {
 namespace kv8 {
 
 constexpr uint32_t T_S = 0, T_O = 256;          // tensor memory: two S buffers of 128 columns, O
-constexpr float LAG = 3.0f, LIFT = 5.0f;        // 2^(LAG + LIFT) = 256 <= 448
+constexpr float LAG = 3.0f;                     // 2^(LAG + LIFT) = 256 <= 448
 constexpr uint32_t SM_WARPS = 16, W_K = 16, W_V = 17, W_MMA = 18, THREADS = 19 * 32;
 // B_P_FULL of a tile counts its softmax warps and the bytes of its first V unit; B_V2_FULL those of a canvas tile's second
 enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V2_FULL = 8, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 13, N_BARS = 15 };
@@ -469,6 +469,24 @@ cudaError_t configure_attn() {
   return e;
 }
 
+cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const uint32_t rows = p.C * p.Hq * (p.D / 256u);
+  if (most_splits > 4) {
+    cfg.gridDim = dim3(rows, p.n_seq);
+    return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<8>, p);
+  }
+  cfg.gridDim = dim3((rows + 7u) / 8u, p.n_seq);
+  return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<1>, p);
+}
+
 cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_ctas);
@@ -480,17 +498,8 @@ cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t mos
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = p.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<512>, p);
-  if (e != cudaSuccess || most_splits == 1) return e;
-  const uint32_t rows = p.C * p.Hq * (p.D / 256u);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  if (most_splits > 4) {
-    cfg.gridDim = dim3(rows, p.n_seq);
-    return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<8>, p);
-  }
-  cfg.gridDim = dim3((rows + 7u) / 8u, p.n_seq);
-  return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<1>, p);
+  const cudaError_t e = p.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<512>, p);
+  return e != cudaSuccess || most_splits == 1 ? e : launch_merge(p, most_splits, st);
 }
 
 }  // namespace kv8
