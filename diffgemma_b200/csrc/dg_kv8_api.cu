@@ -243,10 +243,11 @@ kv8::QueryParams query_params(const dg_layer_desc& d, uint8_t* ws, const RowsLay
 // merge, 2 us and the partial rows' way through memory, 0.33 ns for each row and split.  One canvas of 256 rows, us: 32,768 keys
 // of 2 KV heads, splits 1 / 2 / 3 / 4 / 5 / 7 / 9: 396 / 216 / 158 / 125 / 194 / 160 / 150; window 1024 of 8 KV heads,
 // 1 / 2 / 3 / 4 / 6: 44 / 42 / 38 / 36 / 50; one token over 333 keys, 1 / 2 / 3: 26 / 21 / 19.
-// Single tokens (dg_kv8_token_kernel), all dims in one CTA: what a wave costs beside its tiles is TOKEN_FIXED.
-constexpr uint32_t kFixed8 = 10, kFixedToken = 6;
-uint32_t plan_splits(const dg_ctx* c, kv8::Seq* seq, uint32_t n_seq, uint32_t base, uint64_t rows, uint32_t fixed, const uint32_t* cost,
-                     uint32_t* most_splits) {
+// Single tokens (dg_kv8_token_kernel) have all dims in one CTA and shorter tiles (1 us and less); the merge is a second launch of
+// 3 us behind 10.
+constexpr uint32_t kFixed8 = 10, kFixedToken = 6, kMerge8 = 1400, kMergeToken = 3500;
+uint32_t plan_splits(const dg_ctx* c, kv8::Seq* seq, uint32_t n_seq, uint32_t base, uint64_t rows, uint32_t fixed, uint32_t merge,
+                     const uint32_t* cost, uint32_t* most_splits) {
   const uint32_t sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u;
   uint32_t most = 1;
   for (uint32_t b = 0; b < n_seq; ++b) most = cost[b] > most ? cost[b] : most;
@@ -257,7 +258,7 @@ uint32_t plan_splits(const dg_ctx* c, kv8::Seq* seq, uint32_t n_seq, uint32_t ba
     uint64_t ctas = 0;
     for (uint32_t b = 0; b < n_seq; ++b) ctas += uint64_t(base) * (cost[b] <= per ? 1u : (cost[b] + per - 1) / per);
     const uint64_t waves = (ctas + sms - 1) / sms;
-    const uint64_t t = waves * (per + fixed) * 1000 + (S == 1 ? 0 : 1400 + rows * S * 23 / 100);
+    const uint64_t t = waves * (per + fixed) * 1000 + (S == 1 ? 0 : merge + rows * S * 23 / 100);
     if (t < best_cost) {
       best_cost = t;
       best = per;
@@ -338,7 +339,8 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
     }
     uint32_t splits = 1;
     const uint64_t rows = uint64_t(n) * C * d->n_q_heads * KU;
-    const uint32_t ctas = plan_splits(c, p.seq, n, token ? p.Hkv : p.Hkv * MT * KU, rows, token ? kFixedToken : kFixed8, cost, &splits);
+    const uint32_t ctas = plan_splits(c, p.seq, n, token ? p.Hkv : p.Hkv * MT * KU, rows, token ? kFixedToken : kFixed8, token ? kMergeToken : kMerge8,
+                                      cost, &splits);
     if (splits > 1) {
       const size_t slots = size_t(ctas) * (token ? KU : 1u) * BLK;
       r = grow_bytes(c, &c->kv8_part, &c->kv8_part_bytes, slots * (256 * sizeof(float) + sizeof(float2)));

@@ -407,51 +407,70 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
   if (warp == W_MMA) tmem_dealloc(tmem, 512);
 }
 
-// Splits of a row joined: a row's 256 columns by WARPS warps, each a run of the splits in order, then the warps in order.  One
-// warp a row where the splits are few (and the rows many), eight where they are many.  A split without keys has m = -inf.
+// Splits of a row joined: a row's 256 columns by WARPS warps, each a run of the splits in order, then the warps in order.  A
+// warp's sums stand at the largest reference of its own splits until the warps meet: one round trip to memory.  One warp a row
+// where the splits are few (and the rows many).  A split without keys has m = -inf and l = 0.
 template <uint32_t WARPS>
-__global__ void __launch_bounds__(256) dg_kv8_merge_kernel(const __grid_constant__ AttnParams8 p) {
-  __shared__ float part[8][264];
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) dg_kv8_merge_kernel(const __grid_constant__ AttnParams8 p) {
+  __shared__ float part[WARPS][256];
+  __shared__ float2 ml_w[WARPS];
   grid_launch_dependents();
   grid_wait();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, w = warp % WARPS, b = blockIdx.y, KU = p.D / 256u;
   const Seq& sq = p.seq[b];
-  const uint32_t x = blockIdx.x * (8u / WARPS) + warp / WARPS;
+  const uint32_t x = WARPS == 1 ? blockIdx.x * 8u + warp : blockIdx.x;
   if (sq.n_splits == 1 || x >= p.C * p.Hq * KU) return;      // (whole CTAs where warps work together)
   const uint32_t z = x % KU, row = x / KU, i = row / p.Hq, h = row % p.Hq, kvh = h / p.G;
   const uint32_t R = i * p.G + h % p.G, mt = R / BLK, r = R % BLK, S = sq.n_splits;
   const uint32_t stride = p.Hkv * p.MT * KU, first = sq.first_cta + (kvh * p.MT + mt) * KU + z;
-  float m = -INFINITY;
-  for (uint32_t s = lane; s < S; s += 32u) m = fmaxf(m, p.ws_ml[size_t(first + s * stride) * BLK + r].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const uint32_t s1 = (w + 1) * S / WARPS;
-#pragma unroll 4
-  for (uint32_t s = w * S / WARPS; s < s1; ++s) {
-    const size_t at = size_t(first + s * stride) * BLK + r;
-    const float2 ml = p.ws_ml[at];
-    const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * 256u + lane * 8u);
-    const float4 a = src[0], c = src[1];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float f = fast_exp2(ml.x - m);
-    l = fmaf(f, ml.y, l);
-    acc[0] = fmaf(f, a.x, acc[0]); acc[1] = fmaf(f, a.y, acc[1]); acc[2] = fmaf(f, a.z, acc[2]); acc[3] = fmaf(f, a.w, acc[3]);
-    acc[4] = fmaf(f, c.x, acc[4]); acc[5] = fmaf(f, c.y, acc[5]); acc[6] = fmaf(f, c.z, acc[6]); acc[7] = fmaf(f, c.w, acc[7]);
+  for (uint32_t s = w * S / WARPS; s < s1; s += 4) {
+    float2 ml[4];
+    float4 o[4][2];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const size_t at = size_t(first + (s + k < s1 ? s + k : s) * stride) * BLK + r;
+      const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * 256u + lane * 8u);
+      ml[k] = s + k < s1 ? p.ws_ml[at] : make_float2(-INFINITY, 0.f);
+      o[k][0] = src[0];
+      o[k][1] = src[1];
+    }
+    const float top = fmaxf(fmaxf(m, ml[0].x), fmaxf(ml[1].x, fmaxf(ml[2].x, ml[3].x)));
+    const float keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    l *= keep;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;
+      const float f = ml[k].x == -INFINITY ? ml[k].y : fast_exp2(ml[k].x - top);   // no reference but a sum: not a number
+      l = fmaf(f, ml[k].y, l);
+      acc[0] = fmaf(f, o[k][0].x, acc[0]); acc[1] = fmaf(f, o[k][0].y, acc[1]); acc[2] = fmaf(f, o[k][0].z, acc[2]); acc[3] = fmaf(f, o[k][0].w, acc[3]);
+      acc[4] = fmaf(f, o[k][1].x, acc[4]); acc[5] = fmaf(f, o[k][1].y, acc[5]); acc[6] = fmaf(f, o[k][1].z, acc[6]); acc[7] = fmaf(f, o[k][1].w, acc[7]);
+    }
+    m = top;
   }
   const size_t orow = (size_t(b) * p.C + i) * p.Hq + h;
   if (WARPS > 1) {
     *reinterpret_cast<float4*>(&part[warp][lane * 8u]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     *reinterpret_cast<float4*>(&part[warp][lane * 8u + 4u]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    if (lane == 0) part[warp][256] = l;
+    if (lane == 0) ml_w[warp] = make_float2(m, l);
     __syncthreads();
-    l = 0.f;
-    float y = 0.f;
+    if (threadIdx.x >= 256u) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t k = 0; k < WARPS; ++k) top = fmaxf(top, ml_w[k].x);
+    float sum = 0.f, y = 0.f;
 #pragma unroll
     for (uint32_t k = 0; k < WARPS; ++k) {
-      l += part[k][256];
-      y += part[k][threadIdx.x];
+      if (ml_w[k].x == -INFINITY && ml_w[k].y == 0.f) continue;
+      const float f = ml_w[k].x == -INFINITY ? ml_w[k].y : fast_exp2(ml_w[k].x - top);
+      sum = fmaf(f, ml_w[k].y, sum);
+      y = fmaf(f, part[k][threadIdx.x], y);
     }
+    m = top;
+    l = sum;
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
     p.out[orow * p.D + z * 256u + threadIdx.x] = __float2bfloat16(y * inv);
   } else {
@@ -481,6 +500,10 @@ cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_
   const uint32_t rows = p.C * p.Hq * (p.D / 256u);
   if (most_splits > 4) {
     cfg.gridDim = dim3(rows, p.n_seq);
+    if (most_splits > 16) {
+      cfg.blockDim = dim3(512);
+      return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<16>, p);
+    }
     return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<8>, p);
   }
   cfg.gridDim = dim3((rows + 7u) / 8u, p.n_seq);

@@ -45,7 +45,8 @@ template <uint32_t D> struct TCfg {
 struct Small {
   float c[NR];                        // (by slot) scale * log2 e * 2^exponent of the row
   float red[8][HR];                   // row maxima, row sums by warp
-  float sc[NR][TOKEN_CANVAS];         // canvas scores in base 2
+  float sc[NR][TOKEN_CANVAS];         // canvas scores in base 2, then weights
+  float m0[NR], l0[NR];               // (by slot) reference and sum that a row starts from
   uint32_t lo[NR];                    // (by slot) first cached key that the row sees
 };
 static_assert(sizeof(Small) <= 1024 + 512, "small arrays");
@@ -161,14 +162,9 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
       const size_t q_at = ((size_t(b) * p.C + c) * p.Hq + kvh * p.G + x % p.G) * D + 8u * lane;
       if (live) {
         if (y != warp) request(y);
-        if (is_q || is_k)
-          row_to_bf16<double, NJ>(raw, is_q ? p.qw : p.kw, true, p.eps, p.rope, p.rope.half ? tab + c * p.rope.half : nullptr, lane, v);
-        else if (p.v_norm)
-          row_to_bf16<double, NJ>(raw, nullptr, true, p.eps, p.rope, nullptr, lane, v);
-        else {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) v[j] = raw[j];
-        }
+        const bool turn = (is_q || is_k) && p.rope.half != 0u;
+        row_to_bf16<double, NJ>(raw, is_q ? p.qw : is_k ? p.kw : nullptr, is_q || is_k || p.v_norm != 0u, p.eps, p.rope,
+                                turn ? tab + c * p.rope.half : nullptr, lane, v);
       }
       if (!is_q) {
         uint8_t* dst = smem + (is_k ? cf::O_KB : cf::O_VB) + c * D * 2;
@@ -230,44 +226,45 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
         if (lane == 0) sm.sc[r][c] = t >= rv.can_lo && t < rv.can_hi ? dot * p.scale_log2 : -INFINITY;
       }
       bar_threads(2, PREP_WARPS * 32);
-      if (warp < 8) {
-        float acc[D / 128][HR];
-#pragma unroll
-        for (uint32_t d = 0; d < D / 128; ++d)
-#pragma unroll
-          for (uint32_t j = 0; j < HR; ++j) acc[d][j] = 0.f;
-#pragma unroll
-        for (uint32_t j = 0; j < HR; ++j) {
-          if (j >= nj) continue;
-          const float* sc = sm.sc[2u * j + half];
-          float top = -INFINITY;
-          bool nan = false;
-          for (uint32_t c = 0; c < p.C; ++c) {
-            top = fmaxf(top, sc[c]);
-            nan = nan || sc[c] != sc[c];
-          }
-          m[j] = top;
-          float sum = nan ? __uint_as_float(0x7fc00000u) : 0.f;
-          for (uint32_t c = 0; c < p.C; ++c) {
-            const float w = top == -INFINITY ? 0.f : fast_exp2(sc[c] - top + TLIFT);
-            sum += w;
-#pragma unroll
-            for (uint32_t d = 0; d < D / 128; ++d)
-              acc[d][j] = fmaf(w, __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(smem + cf::O_VB + (c * D + d * 128u + key) * 2u)), acc[d][j]);
-          }
-          l[j] = key == 0 ? sum : 0.f;
+      // a row's weights over the canvas, from which its sums start
+      if (tid < rows) {
+        float* sc = sm.sc[tid];
+        float top = -INFINITY, sum = 0.f;
+        for (uint32_t c = 0; c < p.C; ++c) top = fmaxf(top, sc[c]);
+        for (uint32_t c = 0; c < p.C; ++c) {
+          const float w = sc[c] == -INFINITY ? 0.f : fast_exp2(sc[c] - (top == -INFINITY ? 0.f : top) + TLIFT);   // (NaN stays)
+          sum += w;
+          sc[c] = w;
         }
-#pragma unroll
+        sm.m0[slot_of(tid)] = top;
+        sm.l0[slot_of(tid)] = sum;
+      }
+      bar_threads(2, PREP_WARPS * 32);
+      if (warp < 8) {
+#pragma unroll 1
         for (uint32_t d = 0; d < D / 128; ++d) {
           uint32_t o[8];
+          float acc[HR] = {};
+          for (uint32_t c = 0; c < p.C; ++c) {
+            const float v = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(smem + cf::O_VB + (c * D + d * 128u + key) * 2u));
 #pragma unroll
-          for (uint32_t j = 0; j < HR; ++j) o[j] = __float_as_uint(acc[d][j]);
+            for (uint32_t j = 0; j < HR; ++j)
+              if (j < nj) acc[j] = fmaf(sm.sc[2u * j + half][c], v, acc[j]);
+          }
+#pragma unroll
+          for (uint32_t j = 0; j < HR; ++j) o[j] = __float_as_uint(acc[j]);
           tmem_st8(t_lane + TT_O + d * NO + half * HR, o);
 #pragma unroll
           for (uint32_t j = 0; j < HR; ++j) o[j] = 0u;
 #pragma unroll
           for (uint32_t i = 1; i < TERMS; ++i) tmem_st8(t_lane + TT_O + d * NO + i * NR + half * HR, o);
         }
+#pragma unroll
+        for (uint32_t j = 0; j < HR; ++j)
+          if (j < nj) {
+            m[j] = sm.m0[half * HR + j];
+            l[j] = key == 0 ? sm.l0[half * HR + j] : 0.f;
+          }
         tmem_wait_st();
         tc_fence_before();
       }

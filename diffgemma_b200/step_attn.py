@@ -58,6 +58,14 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr())
 
 
+def _addr(t):
+    """A tensor's address as the C ABI takes it (None: NULL)."""
+    if t is None:
+        return None
+    assert t.is_contiguous(), "tensors handed to the C ABI must be contiguous"
+    return t.data_ptr()
+
+
 class Context:
     """dg_ctx: one per host thread / stream."""
 
@@ -223,8 +231,10 @@ class KvCache8:
         self.ctx = ctx
         self.layer = layer
         self.desc = layer.c_desc()
+        self._desc_ref = C.byref(self.desc)
+        self._device = torch.device("cuda", ctx.device)
         h = C.c_void_p()
-        check(ctx.lib.dg_kv8_create(ctx.h, C.byref(self.desc), capacity_tokens, C.byref(h)), "dg_kv8_create")
+        check(ctx.lib.dg_kv8_create(ctx.h, self._desc_ref, capacity_tokens, C.byref(h)), "dg_kv8_create")
         self.h = h
         ctx._dependents.add(self)
 
@@ -240,22 +250,26 @@ class KvCache8:
     def append(self, k: torch.Tensor, v: torch.Tensor, n_keys: int, pos: int | None = None, kw: torch.Tensor | None = None) -> None:
         """Raw k, v [n, Hkv, D] into slots [n_keys, n_keys + n): norm, RoPE at positions pos.. (None: n_keys), 8 bits."""
         n = self._rows(k, v)
-        check(self.ctx.lib.dg_kv8_append(self.ctx.h, C.byref(self.desc), self.h, n_keys, n_keys if pos is None else pos, n, _ptr(k),
-                                         _ptr(v), _ptr(kw)), "dg_kv8_append")
+        st = self.ctx.lib.dg_kv8_append(self.ctx.h, self._desc_ref, self.h, n_keys, n_keys if pos is None else pos, n, _addr(k), _addr(v),
+                                        _addr(kw))
+        if st:
+            check(st, "dg_kv8_append")
 
     def load(self, k: torch.Tensor, v: torch.Tensor, n_keys: int = 0) -> None:
         """Rows that are ready (K normed and rotated already) into slots [n_keys, n_keys + n)."""
         n = self._rows(k, v)
         if n:
-            check(self.ctx.lib.dg_kv8_load(self.h, n_keys, n, _ptr(k), _ptr(v)), "dg_kv8_load")
+            check(self.ctx.lib.dg_kv8_load(self.h, n_keys, n, _addr(k), _addr(v)), "dg_kv8_load")
 
     def read(self, slot0: int, n: int):
         """Slots [slot0, slot0 + n) as bf16 k, v [n, Hkv, D]."""
         lay = self.layer
-        k = torch.empty((n, lay.n_kv_heads, lay.head_dim), dtype=torch.bfloat16, device=f"cuda:{self.ctx.device}")
+        k = torch.empty((n, lay.n_kv_heads, lay.head_dim), dtype=torch.bfloat16, device=self._device)
         v = torch.empty_like(k)
         if n:
-            check(self.ctx.lib.dg_kv8_read(self.h, _ptr(k), _ptr(v), slot0, n), "dg_kv8_read")
+            st = self.ctx.lib.dg_kv8_read(self.h, _addr(k), _addr(v), slot0, n)
+            if st:
+                check(st, "dg_kv8_read")
         return k, v
 
     def evict_to(self, to: "KvCache8", n_keys: int, weights: torch.Tensor, n_keep: int, n_recent: int = 0, kept=None, weights_out=None):
@@ -266,8 +280,10 @@ class KvCache8:
             kept = torch.empty((heads, n_keep), dtype=torch.int32, device=weights.device)
         assert weights.dtype == torch.float32 and weights.shape[0] == heads and kept.shape == (heads, n_keep)
         assert weights_out is None or (weights_out.dtype == torch.float32 and weights_out.shape[0] == heads)
-        check(self.ctx.lib.dg_kv8_evict(self.ctx.h, self.h, n_keys, _ptr(weights), weights.shape[1], n_keep, n_recent, to.h, _ptr(kept),
-                                        _ptr(weights_out), 0 if weights_out is None else weights_out.shape[1]), "dg_kv8_evict")
+        st = self.ctx.lib.dg_kv8_evict(self.ctx.h, self.h, n_keys, _addr(weights), weights.shape[1], n_keep, n_recent, to.h, _addr(kept),
+                                       _addr(weights_out), 0 if weights_out is None else weights_out.shape[1])
+        if st:
+            check(st, "dg_kv8_evict")
         return kept
 
     def close(self) -> None:
@@ -289,6 +305,8 @@ class CanvasAttention:
         self.ctx = ctx
         self.layer = layer
         self.desc = layer.c_desc()
+        self._desc_ref = C.byref(self.desc)
+        self._batch_arrays = {}
         self.lib = ctx.lib
 
     @property
@@ -333,17 +351,33 @@ class CanvasAttention:
         alone); n_keys and pos: cached tokens and first position of each canvas (pos None: n_keys).  Returns out, or a tuple
         with lse [B,C,Hq] and the rotated queries behind it where asked for."""
         B, lay = len(kvs), self.layer
-        assert q.dtype == torch.bfloat16 and q.shape == (B, lay.canvas, lay.n_q_heads, lay.head_dim)
-        assert (k is None) == (v is None) and (k is None or k.shape == v.shape == (B, lay.canvas, lay.n_kv_heads, lay.head_dim))
-        out = torch.empty_like(q) if out is None else out
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
+        rows = (B, lay.canvas, lay.n_q_heads)
+        assert q.dtype is torch.bfloat16 and q.shape == (*rows, lay.head_dim)
+        if k is not None or v is not None:
+            assert k.shape == v.shape == (B, lay.canvas, lay.n_kv_heads, lay.head_dim) and k.dtype is v.dtype is torch.bfloat16
+        if out is None:
+            out = torch.empty_like(q)
+        lse = q.new_empty(rows, dtype=torch.float32) if with_lse else None
         q_rot = torch.empty_like(q) if with_q_rot else None
-        check(self.lib.dg_kv8_denoise(self.ctx.h, C.byref(self.desc), (C.c_void_p * B)(*[kv.h for kv in kvs]), (C.c_uint32 * B)(*n_keys),
-                                      None if pos is None else (C.c_uint64 * B)(*pos), B, _ptr(q), _ptr(k), _ptr(v), _ptr(qw), _ptr(kw),
-                                      _ptr(out), _ptr(lse), _ptr(q_rot)), "dg_kv8_denoise")
-        if not (with_lse or with_q_rot):
+        handles, lens, places = self._arrays(B)
+        handles[:] = [kv.h.value for kv in kvs]
+        lens[:] = n_keys
+        if pos is not None:
+            places[:] = pos
+        st = self.lib.dg_kv8_denoise(self.ctx.h, self._desc_ref, handles, lens, None if pos is None else places, B, _addr(q), _addr(k),
+                                     _addr(v), _addr(qw), _addr(kw), _addr(out), _addr(lse), _addr(q_rot))
+        if st:
+            check(st, "dg_kv8_denoise")
+        if lse is None and q_rot is None:
             return out
         return tuple(t for t in (out, lse, q_rot) if t is not None)
+
+    def _arrays(self, B: int):
+        """Host arrays of a batch's cache handles, lengths and positions (read by the call before it returns)."""
+        got = self._batch_arrays.get(B)
+        if got is None:
+            got = self._batch_arrays[B] = ((C.c_void_p * B)(), (C.c_uint32 * B)(), (C.c_uint64 * B)())
+        return got
 
     def key_weights(self, kv: KvCache8, n_keys: int, q_rot, lse, weights, decay: float = 1.0):
         """weights = decay * weights + what each cached key drew of the softmax of these rows (dg_kv8_key_weights).  q_rot
@@ -351,8 +385,10 @@ class CanvasAttention:
         lay = self.layer
         assert q_rot.dtype == torch.bfloat16 and q_rot.shape[-3:] == (lay.canvas, lay.n_q_heads, lay.head_dim)
         assert lse.dtype == weights.dtype == torch.float32 and weights.shape[0] == lay.n_kv_heads
-        check(self.lib.dg_kv8_key_weights(self.ctx.h, C.byref(self.desc), kv.h, n_keys, _ptr(q_rot), _ptr(lse), _ptr(weights),
-                                          weights.shape[1], decay), "dg_kv8_key_weights")
+        st = self.lib.dg_kv8_key_weights(self.ctx.h, self._desc_ref, kv.h, n_keys, _addr(q_rot), _addr(lse), _addr(weights),
+                                         weights.shape[1], decay)
+        if st:
+            check(st, "dg_kv8_key_weights")
         return weights
 
     def denoise_host(self, kvs, kv_lens, q, k, v, out, qw=None, kw=None):
