@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(CT, 2) dg_kv8_append_kernel(const __grid_const
   constexpr uint32_t D = 256u * NJ, RW = 8u / NJ, TOK = 16u * RW;     // rows of a warp, tokens of a CTA
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[16];
+  __shared__ __align__(16) float weight[D];
   float2* tab = reinterpret_cast<float2*>(smem);
   grid_launch_dependents();
   grid_wait();
@@ -284,7 +285,11 @@ __global__ void __launch_bounds__(CT, 2) dg_kv8_append_kernel(const __grid_const
       }
     }
   }
-  const bool turn = is_k && !p.ready && p.rope.half != 0u, norm = !p.ready && (is_k || p.v_norm);
+  const bool turn = is_k && !p.ready && p.rope.half != 0u, norm = !p.ready && (is_k || p.v_norm), weighed = norm && is_k && p.kw != nullptr;
+  if (weighed) {
+    if (threadIdx.x < D) weight[threadIdx.x] = __bfloat162float(p.kw[threadIdx.x]);
+    if (!turn) __syncthreads();
+  }
   // a thread's pair and its run of the pass's tokens
   const uint32_t groups = turn ? CT / p.rope.half : 1u, per = (APASS + groups - 1u) / groups;
   const uint32_t dim = turn ? threadIdx.x % p.rope.half : 0u, tok = turn ? threadIdx.x / p.rope.half * per : APASS;
@@ -315,20 +320,29 @@ __global__ void __launch_bounds__(CT, 2) dg_kv8_append_kernel(const __grid_const
       __syncthreads();
     }
     if (r < n_rows && r >= kept) {
-      if (turn || norm) {
+      const float2* cs = turn ? tab + (r % APASS) * p.rope.half : nullptr;
+      if (NJ == 2 && turn && p.rope.dist != 256u) {
         uint4 y[NJ];
-        row_to_bf16<float, NJ>(held[s], is_k ? p.kw : nullptr, norm, p.eps, p.rope, turn ? tab + (r % APASS) * p.rope.half : nullptr, lane, y);
+        row_to_bf16<float, NJ>(held[s], p.kw, true, p.eps, p.rope, cs, lane, y);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) held[s][j] = y[j];
+      } else if (turn || norm) {
+        row_to_bf16_f32<NJ>(held[s], weighed ? weight : nullptr, norm, p.eps, p.rope, cs, lane);
       }
+    }
+    uint32_t big = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) big = abs_max2(abs_max2(abs_max2(abs_max2(big, held[s][j].x), held[s][j].y), held[s][j].z), held[s][j].w);
+    if ((big & 0x7f80u) == 0x7f80u || big >= 0x7f800000u) {    // something is not finite
+      big = 0;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         uint4& y = held[s][j];
         y = make_uint4(finite_or_zero(y.x, &bad), finite_or_zero(y.y, &bad), finite_or_zero(y.z, &bad), finite_or_zero(y.w, &bad));
+        big = abs_max2(abs_max2(abs_max2(abs_max2(big, y.x), y.y), y.z), y.w);
       }
     }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) top = abs_max2(abs_max2(abs_max2(abs_max2(top, held[s][j].x), held[s][j].y), held[s][j].z), held[s][j].w);
+    top = abs_max2(top, big);
   }
   float t = max_of_halves(top);
 #pragma unroll
@@ -345,13 +359,13 @@ __global__ void __launch_bounds__(CT, 2) dg_kv8_append_kernel(const __grid_const
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
   const int e = scale_exp(t);
-  const float mul = pow2i(-e);
+  const uint32_t mul = (__float_as_uint(pow2i(-e)) >> 16) * 0x10001u;
 #pragma unroll
   for (uint32_t s = 0; s < RW; ++s) {
     const uint32_t r = row(s);
     if (r >= n_rows) continue;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) *reinterpret_cast<uint2*>(codes + code8_off(r, lane + 32u * j)) = code8(held[s][j], mul, nullptr);
+    for (int j = 0; j < NJ; ++j) *reinterpret_cast<uint2*>(codes + code8_off(r, lane + 32u * j)) = code8_fast(held[s][j], mul);
   }
   if (bad) dev_status_set(p.status, DG_DEV_NOT_FINITE, KID_CODE, blockIdx.x, t0);
   if (NJ > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves while its maximum may be read

@@ -113,6 +113,85 @@ __device__ __forceinline__ void row_to_bf16(const uint4 (&raw)[NJ], const __nv_b
   }
 }
 
+// The same in 32 bits, by pairs: rows that are appended, whose time is their instructions.  w: the norm's weights as fp32 in
+// shared memory (null: unit).  head_dim 512: pairs 256 apart only.
+template <int NJ>
+__device__ __forceinline__ void row_to_bf16_f32(uint4 (&row)[NJ], const float* w, bool norm, float eps, const Rope& rope, const float2* tab, uint32_t lane) {
+  uint64_t x[NJ][4];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    x[j][0] = bf16x2_to_f32x2(row[j].x);
+    x[j][1] = bf16x2_to_f32x2(row[j].y);
+    x[j][2] = bf16x2_to_f32x2(row[j].z);
+    x[j][3] = bf16x2_to_f32x2(row[j].w);
+  }
+  if (norm) {
+    uint64_t s2 = 0ull;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s2 = fma_f32x2(x[j][i], x[j][i], s2);
+    float a, b;
+    unpack_f32x2(s2, a, b);
+    float ss = a + b;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss * (1.0f / (256.0f * NJ)) + eps);
+    const uint64_t inv2 = pack_f32x2(inv, inv);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j][i] = mul_f32x2(x[j][i], inv2);
+      if (w != nullptr) {
+        const ulonglong2* w2 = reinterpret_cast<const ulonglong2*>(w + 8u * (lane + 32u * j));
+        const ulonglong2 wa = w2[0], wb = w2[1];
+        x[j][0] = mul_f32x2(x[j][0], wa.x);
+        x[j][1] = mul_f32x2(x[j][1], wa.y);
+        x[j][2] = mul_f32x2(x[j][2], wb.x);
+        x[j][3] = mul_f32x2(x[j][3], wb.y);
+      }
+    }
+  }
+  if (tab != nullptr) {
+    const uint32_t hc = rope.half >> 3, dc = rope.dist >> 3;
+    if (NJ == 2) {                                             // a pair lies in one lane
+      if (lane < hc) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 p = tab[(2 * i) * hc + lane], q = tab[(2 * i + 1) * hc + lane];
+          const uint64_t c = pack_f32x2(p.x, q.x), sn = pack_f32x2(p.y, q.y), ng = pack_f32x2(-p.y, -q.y), a = x[0][i], b = x[NJ - 1][i];
+          x[0][i] = fma_f32x2(b, ng, mul_f32x2(a, c));
+          x[NJ - 1][i] = fma_f32x2(a, sn, mul_f32x2(b, c));
+        }
+      }
+    } else {
+      const bool first = lane < hc, second = lane >= dc && lane < dc + hc;
+      const uint32_t src = first ? lane + dc : (second ? lane - dc : lane), at = first ? lane : (second ? lane - dc : 0u);
+      const float sign = first ? -1.0f : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float a, b;
+        unpack_f32x2(x[0][i], a, b);
+        const float o0 = __shfl_sync(0xffffffffu, a, int(src)), o1 = __shfl_sync(0xffffffffu, b, int(src));
+        const float2 p = tab[(2 * i) * hc + at], q = tab[(2 * i + 1) * hc + at];
+        if (first || second) x[0][i] = fma_f32x2(pack_f32x2(o0, o1), pack_f32x2(sign * p.y, sign * q.y), mul_f32x2(x[0][i], pack_f32x2(p.x, q.x)));
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    float a, b;
+    unpack_f32x2(x[j][0], a, b);
+    row[j].x = pack_bf16x2(a, b);
+    unpack_f32x2(x[j][1], a, b);
+    row[j].y = pack_bf16x2(a, b);
+    unpack_f32x2(x[j][2], a, b);
+    row[j].z = pack_bf16x2(a, b);
+    unpack_f32x2(x[j][3], a, b);
+    row[j].w = pack_bf16x2(a, b);
+  }
+}
+
 // larger magnitude of each half, as bf16 bits
 __device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7fff7fffu); }
 // a bf16 pair with what is not finite replaced by zero; *bad is set where that happened
@@ -120,6 +199,20 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t u, bool* bad) {
   if ((u & 0x7f80u) == 0x7f80u) { u &= 0xffff0000u; *bad = true; }
   if ((u & 0x7f800000u) == 0x7f800000u) { u &= 0xffffu; *bad = true; }
   return u;
+}
+// a bf16 pair times a power of two (both halves of m): exact
+__device__ __forceinline__ uint32_t scale_bf16x2(uint32_t v, uint32_t m) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(m));
+  return r;
+}
+// eight bf16 times 2^-e, given as a bf16 pair, as e4m3 codes
+__device__ __forceinline__ uint2 code8_fast(const uint4& v, uint32_t m) {
+  const uint32_t u[4] = {scale_bf16x2(v.x, m), scale_bf16x2(v.y, m), scale_bf16x2(v.z, m), scale_bf16x2(v.w, m)};
+  uint16_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+  return make_uint2(uint32_t(h[0]) | (uint32_t(h[1]) << 16), uint32_t(h[2]) | (uint32_t(h[3]) << 16));
 }
 // eight bf16 times 2^-e as e4m3 codes, and the codes of what that rounding left
 __device__ __forceinline__ uint2 code8(const uint4& v, float mul, uint2* rest) {
