@@ -167,7 +167,8 @@ struct Rope {
 };
 
 // rows of canvas queries, coded: [seq][KV head][row tile of 128][term][slab][128 rows][128 B], and per row what its scores
-// are multiplied by (scale * log2 e * 2^row exponent) and, for the key weights, -log2 e * lse
+// are multiplied by (scale * log2 e * 2^row exponent) and, for the key weights, -log2 e * lse (there as pairs of rows: two
+// factors, then two sums)
 struct QueryRows {
   uint8_t* codes;
   float2* row;
@@ -264,11 +265,11 @@ struct WeightParams {
   uint32_t blocks, n_keys;
   uint32_t C, Hkv, G, MT;
   uint32_t mode, windowed, wm1;
+  uint32_t run0;               // the first run of keys that some row sees
   float* w;                    // [Hkv][ld]
   uint64_t ld;
   float decay;
-  float* part;                 // [row split][Hkv][n_keys] when there is more than one
-  uint32_t row_splits;
+  float* part;                 // [piece][Hkv][n_keys] where CTAs share runs of keys, else null
   DevStatus* status;
 };
 
@@ -340,7 +341,7 @@ cudaError_t launch_read(const ReadParams& p, cudaStream_t st);
 cudaError_t launch_token(const TokenParams& p, uint32_t D, uint32_t n_ctas, cudaStream_t st);
 cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_t st);
 cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st);
-cudaError_t launch_weights(const WeightParams& p, uint32_t D, cudaStream_t st);
+cudaError_t launch_weights(const WeightParams& p, uint32_t D, uint32_t ctas, cudaStream_t st);
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st);
 
 }  // namespace kv8

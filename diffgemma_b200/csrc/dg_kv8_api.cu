@@ -466,26 +466,30 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   p.ld = ld;
   p.decay = decay;
   p.status = c->d_status;
-  // few keys: the rows are shared out as well, two CTAs or more for a run of keys, and their sums added in order
+  // One CTA a run of keys where the runs are a whole number of waves or few steps long; else an even cut of all steps, runs shared
+  // at the cuts: 2 steps for what a second launch costs, 2 for what a run or a CTA costs beside its steps (1.2 us each).
   const uint32_t sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u, kt = 512 / D, blocks = (n_keys + BLK - 1) / BLK;
-  const uint32_t grid = (blocks + kt - 1) / kt * p.Hkv, steps = (C * G * (D / 256) + BLK - 1) / BLK;
-  uint64_t best = ~0ull;
-  for (uint32_t s = 1; s <= 8 && s <= steps; ++s) {
-    const uint64_t t = (uint64_t(grid) * s + sms - 1) / sms * ((steps + s - 1) / s + 3) + (s > 1 ? 3 : 0);
-    if (t < best) {
-      best = t;
-      p.row_splits = s;
-    }
+  {
+    MaskParams mk = make_mask(*d, n_keys, 0, n_keys, 0);
+    const uint32_t lo = mask_row_lo(mk, 0), last = (blocks + kt - 1) / kt - 1;
+    p.run0 = lo / BLK / kt < last ? lo / BLK / kt : last;
   }
-  if (p.row_splits > 1) {
-    r = grow_bytes(c, &c->kv8_part, &c->kv8_part_bytes, size_t(p.row_splits) * p.Hkv * n_keys * sizeof(float));
+  const uint32_t runs = ((blocks + kt - 1) / kt - p.run0) * p.Hkv, steps = (C * G * (D / 256) + BLK - 1) / BLK;
+  const uint64_t units = uint64_t(runs) * steps;
+  uint32_t ctas = runs;
+  const uint32_t whole = (runs + sms - 1) / sms * (steps + 2);
+  const uint32_t even = uint32_t(units < sms ? units : sms), per = uint32_t((units + even - 1) / even);
+  if (per + 2u * (per / steps + 1u) + 4u < whole) {
+    ctas = even;
+    const uint32_t pieces = steps / uint32_t(units / even) + 2u;   // CTAs that a run's stages can be spread over
+    r = grow_bytes(c, &c->kv8_part, &c->kv8_part_bytes, size_t(pieces) * p.Hkv * n_keys * sizeof(float));
     if (r != DG_OK) return r;
     p.part = reinterpret_cast<float*>(c->kv8_part);
   }
   const uint64_t at = 0;
   DG_CUDA(kv8::launch_rows(qp, kv8::CodeParams{}, &at, 1, c->stream));
-  DG_CUDA(kv8::launch_weights(p, D, c->stream));
-  c->last_launches = p.row_splits > 1 ? 3 : 2;
+  DG_CUDA(kv8::launch_weights(p, D, ctas, c->stream));
+  c->last_launches = p.part ? 3 : 2;
   return DG_OK;
 }
 

@@ -223,7 +223,14 @@ __global__ void __launch_bounds__(CT, NJ == 1 ? 2 : 1) dg_kv8_rows_kernel(const 
         const float l = q.lse[(size_t(b) * o.C + i) * o.Hq + h];
         nl = l == -INFINITY ? -INFINITY : -1.4426950408889634f * l;
       }
-      o.row[(size_t(b) * o.Hkv + kvh) * o.MT * BLK + R] = make_float2(q.scale_log2 * pow2i(e), nl);
+      const size_t at = (size_t(b) * o.Hkv + kvh) * o.MT * BLK + R;
+      if (q.lse != nullptr) {   // two rows' factors, then their -lse: as pairs
+        float* pair = reinterpret_cast<float*>(o.row) + (at & ~size_t(1)) * 2u + (at & 1u);
+        pair[0] = q.scale_log2 * pow2i(e);
+        pair[2] = nl;
+      } else {
+        o.row[at] = make_float2(q.scale_log2 * pow2i(e), nl);
+      }
     }
   }
 }

@@ -5,7 +5,9 @@
 // of keys in shared memory (256 keys of 256 dims, or 128 of 512) and streams all query rows past them in 64 KB stages (two
 // terms, as in the attention kernel); rows come out of L2, keys out of HBM once.  Per 128 keys, 128 rows and 256 dims:
 // 1,024 cycles of MMA, 16,384 exponentials (1,024 cycles), 32 bytes a cycle of rows.
-// Every key belongs to one thread of one CTA, or of a fixed number of CTAs whose sums are added in order: no atomics.
+// The work is a line of units, (head, run of keys, stage of rows), cut evenly: a CTA has one stretch of it, and the runs of
+// keys at its ends may be shared with its neighbours.  Every key's sum is one thread's, or of a few CTAs whose sums a second
+// launch adds in order: no atomics.
 #include "dg_kv8.cuh"
 
 namespace dg {
@@ -20,7 +22,9 @@ template <uint32_t D> struct WCfg {
   static constexpr uint32_t TM_COLS = 2 * KT * NR;
 };
 constexpr uint32_t W_EPI = 16, WW_LOAD = 16, WW_MMA = 17, W_THREADS = 18 * 32;
-enum { WB_K = 0, WB_Q_FULL = 1, WB_Q_EMPTY = 3, WB_S_FULL = 5, WB_S_EMPTY = 7 };
+// WB_Q_FULL of a stage counts its bytes and the sixteen warps that have read the scores of the stage before last: one wait for
+// the MMA warp.  WB_S_FULL says that the scores are there and the stage is free.
+enum { WB_K = 0, WB_Q_FULL = 1, WB_S_FULL = 3, W_BARS = 5 };
 
 template <uint32_t D>
 __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __grid_constant__ WeightParams p) {
@@ -31,7 +35,6 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
   volatile uint32_t* abort_flag = &ctl[0];
   auto bar = [&](uint32_t i) { return s0 + cf::O_BAR + i * 8u; };
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t kvh = blockIdx.y, rs = blockIdx.z;
   grid_launch_dependents();
   if (s0 & 1023u) {
     if (tid == 0) dev_status_set(p.status, DG_DEV_SMEM_LAYOUT, KID_WEIGHTS, blockIdx.x, s0);
@@ -39,7 +42,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
   }
   if (tid == 0) {
     ctl[0] = 0u;
-    for (uint32_t i = 0; i < 9; ++i) mbar_init(bar(i), i >= WB_S_EMPTY ? W_EPI : 1u);
+    for (uint32_t i = 0; i < W_BARS; ++i) mbar_init(bar(i), i == WB_Q_FULL || i == WB_Q_FULL + 1 ? W_EPI + 1u : 1u);
     fence_mbar_init();
   }
   if (warp == WW_MMA) {
@@ -52,132 +55,180 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
   const uint32_t tmem = ctl[1];
   grid_wait();
 
-  const uint32_t rows = p.C * p.G, n_blocks = (p.n_keys + BLK - 1) / BLK;
-  const uint32_t first = blockIdx.x * cf::KT, have = n_blocks - first < cf::KT ? n_blocks - first : cf::KT;
+  const uint32_t rows = p.C * p.G, n_blocks = (p.n_keys + BLK - 1) / BLK, runs = (n_blocks + cf::KT - 1) / cf::KT - p.run0;
+  const uint32_t steps = (rows + cf::NR - 1) / cf::NR;
   MaskParams mk = {};
   mk.kv_len = mk.pre_hi = mk.can_hi = p.n_keys;
   mk.mode = p.mode;
   mk.windowed = p.windowed;
   mk.wm1 = p.wm1;
-  const uint32_t all_steps = (rows + cf::NR - 1) / cf::NR;
-  const uint32_t st0 = uint32_t(uint64_t(all_steps) * rs / p.row_splits);
-  uint32_t st1 = uint32_t(uint64_t(all_steps) * (rs + 1) / p.row_splits);
-  if ((first + have) * BLK <= mask_row_lo(mk, 0)) st1 = st0;   // nobody sees these keys
-  const uint32_t n_steps = st1 - st0;
-  const size_t q_head = size_t(kvh) * p.MT;
+  const uint64_t units = uint64_t(p.Hkv) * runs * steps;
+  const uint64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1u) / gridDim.x;
   float* red = reinterpret_cast<float*>(smem + cf::O_R);
+  // a CTA's pieces: f(first stage, last + 1, KV head, first block, blocks, piece) for each run of keys that its stretch touches
+  auto each_piece = [&](auto f) {
+    uint32_t piece = 0;
+    for (uint64_t u = u0; u < u1; ++piece) {
+      const uint32_t run = uint32_t(u / steps), st0 = uint32_t(u % steps);
+      const uint64_t end = u1 < uint64_t(run + 1) * steps ? u1 : uint64_t(run + 1) * steps;
+      const uint32_t first = (p.run0 + run % runs) * cf::KT;
+      if (!f(st0, st0 + uint32_t(end - u), run / runs, first, n_blocks - first < cf::KT ? n_blocks - first : cf::KT, piece)) break;
+      u = end;
+    }
+  };
 
   if (warp < W_EPI) {
     const uint32_t quarter = warp & 3u, g = warp >> 2;
     const uint32_t kt = g * cf::COLS / cf::NR, col0 = g * cf::COLS % cf::NR;
-    const uint32_t key = quarter * 32u + lane, t = (first + kt) * BLK + key;
-    const bool live = t < p.n_keys;
-    const float kscale = kt < have ? pow2i(p.exps[size_t(kvh) * p.blocks + first + kt].x) : 0.f;
-    // keys that some row does not see: a look at each row's window
-    const bool edge = (first + kt) * BLK < mask_row_lo(mk, p.C - 1);
-    float acc[2] = {0.f, 0.f};
-    for (uint32_t n = 0; n < n_steps; ++n) {
-      const uint32_t sb = n & 1u;
-      if (!__all_sync(0xffffffffu, bar_wait(bar(WB_S_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
-      tc_fence_after();
-      const float4* cst = reinterpret_cast<const float4*>(smem + cf::O_C + ((n & 3u) * cf::NR + col0) * 8u);
-      const uint32_t src = tmem + ((quarter * 32u) << 16) + sb * (cf::KT * cf::NR) + kt * cf::NR + col0;
-      constexpr uint32_t W = cf::COLS < 32 ? cf::COLS : 32;
-#pragma unroll 1
-      for (uint32_t c = 0; c < cf::COLS; c += W) {
-        uint32_t s[W];
-        if constexpr (W == 32) tmem_ld32(src + c, s); else tmem_ld16(src + c, s);
-        tmem_wait_ld();
-        if (c + W >= cf::COLS) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(WB_S_EMPTY + sb));
+    const uint32_t key = quarter * 32u + lane;
+    constexpr uint32_t W = cf::COLS < 32 ? cf::COLS : 32, CH = cf::COLS / W;
+    uint32_t n = 0;
+    if (lane == 0) {
+      mbar_arrive(bar(WB_Q_FULL));
+      mbar_arrive(bar(WB_Q_FULL + 1));
+    }
+    // keys ahead of every row's window
+    if (p.decay != 1.0f) {
+      const uint32_t behind = p.run0 * cf::KT * BLK;
+      for (uint64_t x = uint64_t(blockIdx.x) * (W_EPI * 32) + tid; x < uint64_t(behind) * p.Hkv; x += uint64_t(gridDim.x) * (W_EPI * 32)) {
+        float* w = p.w + x / behind * p.ld + x % behind;
+        *w = p.decay != 0.f ? p.decay * *w : 0.f;
+      }
+    }
+    each_piece([&](uint32_t st0, uint32_t st1, uint32_t kvh, uint32_t first, uint32_t have, uint32_t) -> bool {
+      const uint32_t t = (first + kt) * BLK + key;
+      const float kscale = kt < have ? pow2i(p.exps[size_t(kvh) * p.blocks + first + kt].x) : 0.f;
+      // keys that some row does not see: a look at each row's window
+      const bool edge = (first + kt) * BLK < mask_row_lo(mk, p.C - 1);
+      uint64_t acc = 0ull;
+      const uint64_t ks2 = pack_f32x2(kscale, kscale);
+      bool ok = true;
+      for (uint32_t st = st0; st < st1; ++st, ++n) {
+        const uint32_t sb = n & 1u;
+        ok = __all_sync(0xffffffffu, bar_wait(bar(WB_S_FULL + sb), (n >> 1) & 1u, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const ulonglong2* cst = reinterpret_cast<const ulonglong2*>(smem + cf::O_C + (n & 3u) * cf::NR * 8u) + col0 / 2u;
+        const uint32_t src = tmem + ((quarter * 32u) << 16) + sb * (cf::KT * cf::NR) + kt * cf::NR + col0;
+        uint32_t s[CH][W];
+#pragma unroll
+        for (uint32_t c = 0; c < CH; ++c) {
+          if constexpr (W == 32) tmem_ld32(src + c * W, s[c]); else tmem_ld16(src + c * W, s[c]);
         }
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(WB_Q_FULL + sb));   // for the stage after next
+        auto weight = [&](uint32_t c, uint32_t e) -> uint64_t {
+          const ulonglong2 k = cst[(c * W + e) >> 1];      // factors and -lse of two rows, one broadcast
+          float x0, x1;
+          unpack_f32x2(fma_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), ks2), k.x, k.y), x0, x1);
+          return pack_f32x2(fast_exp2(x0), fast_exp2(x1));
+        };
         if (!edge) {
 #pragma unroll
-          for (uint32_t e = 0; e < W; e += 2) {
-            const float4 k = cst[(c + e) >> 1];   // (factor, -lse) of two rows, one broadcast
-            acc[0] += fast_exp2(fmaf(__uint_as_float(s[e]) * kscale, k.x, k.y));
-            acc[1] += fast_exp2(fmaf(__uint_as_float(s[e + 1]) * kscale, k.z, k.w));
-          }
-        } else {
+          for (uint32_t c = 0; c < CH; ++c)
 #pragma unroll
-          for (uint32_t e = 0; e < W; e += 2) {
-            const float4 k = cst[(c + e) >> 1];
-            const uint32_t R = (st0 + n) * cf::NR + col0 + c + e;
-            if (t >= mask_row_lo(mk, R / p.G)) acc[0] += fast_exp2(fmaf(__uint_as_float(s[e]) * kscale, k.x, k.y));
-            if (t >= mask_row_lo(mk, (R + 1) / p.G)) acc[1] += fast_exp2(fmaf(__uint_as_float(s[e + 1]) * kscale, k.z, k.w));
-          }
+            for (uint32_t e = 0; e < W; e += 2) acc = add_f32x2(acc, weight(c, e));
+        } else {
+#pragma unroll 1
+          for (uint32_t c = 0; c < CH; ++c)
+#pragma unroll
+            for (uint32_t e = 0; e < W; e += 2) {
+              const uint32_t R = st * cf::NR + col0 + c * W + e;
+              float x0, x1;
+              unpack_f32x2(c == 0 ? weight(0, e) : weight(CH - 1, e), x0, x1);
+              x0 = t >= mask_row_lo(mk, R / p.G) ? x0 : 0.f;
+              x1 = t >= mask_row_lo(mk, (R + 1) / p.G) ? x1 : 0.f;
+              acc = add_f32x2(acc, pack_f32x2(x0, x1));
+            }
         }
       }
-    }
-    red[g * BLK + key] = acc[0] + acc[1];
-    asm volatile("bar.sync 1, %0;" ::"n"(W_EPI * 32) : "memory");
-    // the threads that share a key: the column groups of its tile
-    constexpr uint32_t PER = 4 / cf::KT;
-    if (g % PER == 0 && live && kt < have && !*abort_flag) {
-      float sum = 0.f;
+      float a, b;
+      unpack_f32x2(acc, a, b);
+      red[g * BLK + key] = a + b;
+      asm volatile("bar.sync 1, %0;" ::"n"(W_EPI * 32) : "memory");
+      // the threads that share a key: the column groups of its tile
+      constexpr uint32_t PER = 4 / cf::KT;
+      if (g % PER == 0 && t < p.n_keys && kt < have && ok && !*abort_flag) {
+        float sum = 0.f;
 #pragma unroll
-      for (uint32_t i = 0; i < PER; ++i) sum += red[(g + i) * BLK + key];
-      if (p.row_splits > 1) {
-        p.part[(size_t(rs) * p.Hkv + kvh) * p.n_keys + t] = sum;
-      } else {
-        float* w = p.w + size_t(kvh) * p.ld + t;
-        *w = p.decay != 0.f ? fmaf(p.decay, *w, sum) : sum;
+        for (uint32_t i = 0; i < PER; ++i) sum += red[(g + i) * BLK + key];
+        if (st0 != 0 || st1 != steps) {
+          // a piece of the run's stages: its place is the CTA's distance from the first that has one of them
+          const uint64_t run = uint64_t(kvh) * runs + first / cf::KT - p.run0;
+          const uint32_t owner = uint32_t((run * steps * gridDim.x + gridDim.x) / units);   // CTA with the run's first stage, or the one after
+          const uint32_t lead = units * owner / gridDim.x > run * steps ? owner - 1u : owner;
+          p.part[(size_t(blockIdx.x - lead) * p.Hkv + kvh) * p.n_keys + t] = sum;
+        } else {
+          float* w = p.w + size_t(kvh) * p.ld + t;
+          *w = p.decay != 0.f ? fmaf(p.decay, *w, sum) : sum;
+        }
       }
-    }
+      asm volatile("bar.sync 1, %0;" ::"n"(W_EPI * 32) : "memory");
+      return ok;
+    });
   } else if (warp == WW_LOAD) {
-    if (lane == 0 && n_steps > 0) {
-      mbar_expect_tx(bar(WB_K), have * BLK * D);
-      const uint8_t* k = p.k + (size_t(kvh) * p.blocks + first) * BLK * D;
-      for (uint32_t o = 0; o < have * BLK * D; o += UNIT) bulk_load(s0 + o, k + o, UNIT, bar(WB_K));
-      for (uint32_t n = 0; n < n_steps; ++n) {
-        const uint32_t sb = n & 1u, full = bar(WB_Q_FULL + sb), step = st0 + n;
-        if (n > 1 && !bar_wait(bar(WB_Q_EMPTY + sb), ((n - 2) >> 1) & 1u, abort_flag)) break;
-        // the constants' slot was last read for step n - 4, which S^T of step n - 2 waited for
-        mbar_expect_tx(full, cf::STAGE + cf::NR * 8u);
-        const uint32_t dst = s0 + cf::O_Q + sb * cf::STAGE;
-        const uint32_t R0 = step * cf::NR, mt = R0 / BLK;
-        const uint8_t* q = p.q_codes + (q_head + mt) * 2u * BLK * D;
-        if (cf::NR == BLK) {
-          for (uint32_t o = 0; o < cf::STAGE; o += UNIT) bulk_load(dst + o, q + o, UNIT, full);
-        } else {
-          for (uint32_t sl = 0; sl < 2 * D / 128; ++sl)
-            bulk_load(dst + sl * cf::NR * 128u, q + sl * SLAB + (R0 % BLK) * 128u, cf::NR * 128u, full);
-        }
-        bulk_load(s0 + cf::O_C + (n & 3u) * cf::NR * 8u, p.q_row + q_head * BLK + R0, cf::NR * 8u, full);
-      }
-    }
-  } else if (n_steps > 0) {
-    constexpr uint32_t IDESC = idesc_f8(128, cf::NR, 0, 0);
-    const uint64_t dk = umma_smem_desc(s0, 16, 1024), dq = umma_smem_desc(s0 + cf::O_Q, 16, 1024);
-    bool ok = __all_sync(0xffffffffu, bar_wait(bar(WB_K), 0u, abort_flag));
-    for (uint32_t n = 0; ok && n < n_steps; ++n) {
-      const uint32_t sb = n & 1u;
-      if (n > 1 && !__all_sync(0xffffffffu, bar_wait(bar(WB_S_EMPTY + sb), ((n - 2) >> 1) & 1u, abort_flag))) break;
-      if (!__all_sync(0xffffffffu, bar_wait(bar(WB_Q_FULL + sb), (n >> 1) & 1u, abort_flag))) break;
-      tc_fence_after();
-      if (elect_one()) {
-#pragma unroll 1
-        for (uint32_t kt = 0; kt < cf::KT; ++kt) {
-          const uint32_t d_tmem = tmem + sb * (cf::KT * cf::NR) + kt * cf::NR;
-#pragma unroll 1
-          for (uint32_t ts = 0; ts < 2 * D / 128; ++ts) {   // term and slab of the rows
-            const uint64_t qb = dq + uint64_t((sb * cf::STAGE + ts * cf::NR * 128u) >> 4);
-            const uint64_t ka = dk + uint64_t((kt * BLK * D + (ts % (D / 128)) * SLAB) >> 4);
-#pragma unroll
-            for (uint32_t kk = 0; kk < 4; ++kk) mma_ss(d_tmem, ka + kk * 2u, qb + kk * 2u, IDESC, (ts | kk) != 0u);
+    if (lane == 0) {
+      uint32_t n = 0;
+      each_piece([&](uint32_t st0, uint32_t st1, uint32_t kvh, uint32_t first, uint32_t have, uint32_t) -> bool {
+        // the keys' place is free when the last products with them are done
+        if (n != 0 && !bar_wait(bar(WB_S_FULL + ((n - 1u) & 1u)), ((n - 1u) >> 1) & 1u, abort_flag)) return false;
+        mbar_expect_tx(bar(WB_K), have * BLK * D);
+        const uint8_t* k = p.k + (size_t(kvh) * p.blocks + first) * BLK * D;
+        for (uint32_t o = 0; o < have * BLK * D; o += UNIT) bulk_load(s0 + o, k + o, UNIT, bar(WB_K));
+        for (uint32_t st = st0; st < st1; ++st, ++n) {
+          const uint32_t sb = n & 1u, full = bar(WB_Q_FULL + sb);
+          if (n > 1 && !bar_wait(bar(WB_S_FULL + sb), ((n - 2) >> 1) & 1u, abort_flag)) return false;
+          // the constants' slot was last read for step n - 4, which S^T of step n - 2 waited for
+          mbar_expect_tx(full, cf::STAGE + cf::NR * 8u);
+          const uint32_t dst = s0 + cf::O_Q + sb * cf::STAGE;
+          const uint32_t R0 = st * cf::NR, mt = R0 / BLK;
+          const uint8_t* q = p.q_codes + (size_t(kvh) * p.MT + mt) * 2u * BLK * D;
+          if (cf::NR == BLK) {
+            for (uint32_t o = 0; o < cf::STAGE; o += UNIT) bulk_load(dst + o, q + o, UNIT, full);
+          } else {
+            for (uint32_t sl = 0; sl < 2 * D / 128; ++sl)
+              bulk_load(dst + sl * cf::NR * 128u, q + sl * SLAB + (R0 % BLK) * 128u, cf::NR * 128u, full);
           }
+          bulk_load(s0 + cf::O_C + (n & 3u) * cf::NR * 8u, p.q_row + size_t(kvh) * p.MT * BLK + R0, cf::NR * 8u, full);
         }
-        umma_commit(bar(WB_Q_EMPTY + sb));
-        umma_commit(bar(WB_S_FULL + sb));
-      }
-      __syncwarp();
+        return true;
+      });
     }
+  } else {
+    constexpr uint32_t IDESC = idesc_f8(128, cf::NR, 0, 0);
+    constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+    auto desc = [](uint32_t lo) { return (uint64_t(HI) << 32) | uint64_t(lo); };
+    const uint32_t dk = ((s0 >> 4) & 0x3fffu) | (1u << 16), dq = (((s0 + cf::O_Q) >> 4) & 0x3fffu) | (1u << 16);
+    uint32_t n = 0;
+    each_piece([&](uint32_t st0, uint32_t st1, uint32_t, uint32_t, uint32_t, uint32_t piece) -> bool {
+      if (!__all_sync(0xffffffffu, bar_wait(bar(WB_K), piece & 1u, abort_flag))) return false;
+      for (uint32_t st = st0; st < st1; ++st, ++n) {
+        const uint32_t sb = n & 1u;
+        if (!__all_sync(0xffffffffu, bar_wait(bar(WB_Q_FULL + sb), (n >> 1) & 1u, abort_flag))) return false;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (uint32_t kt = 0; kt < cf::KT; ++kt) {
+            const uint32_t d_tmem = tmem + sb * (cf::KT * cf::NR) + kt * cf::NR;
+#pragma unroll
+            for (uint32_t j = 0; j < 8 * D / 128; ++j) {   // term and slab of the rows, 32 dims
+              const uint32_t ts = j >> 2, kk = j & 3u;
+              mma_ss(d_tmem, desc(dk + ((kt * BLK * D + (ts % (D / 128)) * SLAB) >> 4) + kk * 2u),
+                     desc(dq + sb * (cf::STAGE >> 4) + ((ts * cf::NR * 128u) >> 4) + kk * 2u), IDESC, j != 0 ? 1u : 0u);
+            }
+          }
+          umma_commit(bar(WB_S_FULL + sb));
+        }
+        __syncwarp();
+      }
+      return true;
+    });
   }
 
   if (*abort_flag) {
-    if (tid == 0) dev_status_set(p.status, DG_DEV_WAIT_TIMEOUT, KID_WEIGHTS, blockIdx.x, n_steps);
+    if (tid == 0) dev_status_set(p.status, DG_DEV_WAIT_TIMEOUT, KID_WEIGHTS, blockIdx.x, uint32_t(u1 - u0));
     if (warp == WW_LOAD && lane == 0) {
       const long long c0 = clock64();
       while (clock64() - c0 < 2000000ll) {}
@@ -188,13 +239,20 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
   if (warp == WW_MMA) tmem_dealloc(tmem, cf::TM_COLS);
 }
 
-__global__ void __launch_bounds__(256) dg_kv8_weights_sum_kernel(const __grid_constant__ WeightParams p) {
+// The pieces of runs that several CTAs share, in order.
+__global__ void __launch_bounds__(256) dg_kv8_weights_sum_kernel(const __grid_constant__ WeightParams p, uint32_t ctas, uint32_t run_keys, uint32_t steps) {
   grid_launch_dependents();
   grid_wait();
   const uint32_t t = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y;
-  if (t >= p.n_keys) return;
+  if (t >= p.n_keys || t < p.run0 * run_keys) return;
+  const uint32_t runs = (p.n_keys + run_keys - 1) / run_keys - p.run0;
+  const uint64_t units = uint64_t(p.Hkv) * runs * steps, a = (uint64_t(kvh) * runs + t / run_keys - p.run0) * steps, z = a + steps;
+  // CTA i has units [units * i / ctas, units * (i + 1) / ctas)
+  uint32_t i = uint32_t((a * ctas + ctas) / units);
+  if (units * i / ctas > a) --i;
+  if (units * (i + 1) / ctas >= z) return;         // one CTA has them all
   float sum = 0.f;
-  for (uint32_t s = 0; s < p.row_splits; ++s) sum += p.part[(size_t(s) * p.Hkv + kvh) * p.n_keys + t];
+  for (uint32_t k = 0; i < ctas && units * i / ctas < z; ++i, ++k) sum += p.part[(size_t(k) * p.Hkv + kvh) * p.n_keys + t];
   float* w = p.w + size_t(kvh) * p.ld + t;
   *w = p.decay != 0.f ? fmaf(p.decay, *w, sum) : sum;
 }
@@ -205,10 +263,9 @@ cudaError_t configure_weights() {
   return e;
 }
 
-cudaError_t launch_weights(const WeightParams& p, uint32_t D, cudaStream_t st) {
-  const uint32_t kt = 512 / D, blocks = (p.n_keys + BLK - 1) / BLK;
+cudaError_t launch_weights(const WeightParams& p, uint32_t D, uint32_t ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((blocks + kt - 1) / kt, p.Hkv, p.row_splits);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(W_THREADS);
   cfg.dynamicSmemBytes = D == 256 ? WCfg<256>::SMEM : WCfg<512>::SMEM;
   cfg.stream = st;
@@ -217,12 +274,13 @@ cudaError_t launch_weights(const WeightParams& p, uint32_t D, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_weights_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_weights_kernel<512>, p);
-  if (e != cudaSuccess || p.row_splits == 1) return e;
+  const cudaError_t e = D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_weights_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_weights_kernel<512>, p);
+  if (e != cudaSuccess || p.part == nullptr) return e;
+  const uint32_t nr = D == 256 ? WCfg<256>::NR : WCfg<512>::NR;
   cfg.gridDim = dim3((p.n_keys + 255u) / 256u, p.Hkv);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, dg_kv8_weights_sum_kernel, p);
+  return cudaLaunchKernelEx(&cfg, dg_kv8_weights_sum_kernel, p, ctas, 512 / D * BLK, (p.C * p.G + nr - 1) / nr);
 }
 
 }  // namespace kv8
