@@ -12,11 +12,13 @@ cudaError_t configure_code();
 cudaError_t configure_attn();
 cudaError_t configure_weights();
 cudaError_t configure_token();
+cudaError_t configure_evict();
 cudaError_t configure() {
   cudaError_t e = configure_code();
   if (e == cudaSuccess) e = configure_attn();
   if (e == cudaSuccess) e = configure_weights();
   if (e == cudaSuccess) e = configure_token();
+  if (e == cudaSuccess) e = configure_evict();
   return e;
 }
 }  // namespace kv8

@@ -1,18 +1,22 @@
 // Eviction: the n_recent last tokens of a cache and, of those before them, the n_keep - n_recent with the largest weights
 // (equal ones: lowest index), in order, into another cache.
 //
-// Selection, a cluster of up to eight CTAs for each head: the cut is found exactly by a radix over 32-bit order keys (digits of
-// 11, 11 and 10 bits).  A thread holds its run of up to 16 tokens in registers (131,072 tokens a head; longer rows are read
-// again for each digit).  A CTA counts its part; of the digit's bins each CTA adds up an eighth over the cluster and stores the
-// sums to all (distributed shared memory carries every count once), then each finds the cut for itself, and each thread places
-// its run by the counts ahead of it.  Moving, a CTA for each block of the new cache: 128 gathered rows of codes, whose values
-// get the scale of their new block; the codes stay as they are where the scale does.
+// Selection, a cluster of up to sixteen CTAs for each head: the cut is found exactly by a radix over 32-bit order keys, eight
+// bits a pass.  A lane holds every 32nd token of its warp's stretch in registers, up to 16 of them (262,144 tokens a head; longer
+// rows are read again for each pass), so that loads are whole lines and a token's place comes from ballots.  In a pass a CTA
+// counts its tokens by digit, every CTA reads the counts of all (distributed shared memory, one barrier a pass) and finds the
+// digit for itself; the counts of the CTAs ahead that lie above the cut add up to its first place in the output, so that no
+// exchange follows the last pass.  What bounds it is those barriers and the CTAs that hold the row: 131,072 tokens of 2 heads
+// take 16.7 us (24.1 with 8 CTAs, runs of tokens by thread and digits of 11 bits; counts of a digit aggregated by match or in
+// copies by lane were slower than plain shared-memory adds, which the unit merges: 2,000 cycles a pass against 5,000 and 9,000).
+// Moving, a CTA for each block of the new cache: 128 gathered rows of codes, whose values get the scale of their new block; the
+// codes stay as they are where the scale does.
 #include "dg_kv8.cuh"
 
 namespace dg {
 namespace kv8 {
 
-constexpr uint32_t SEL_T = 1024, BINS = 2048, RUN = 16;
+constexpr uint32_t SEL_T = 1024, BINS = 256, RUN = 16, MAX_CTAS = 16;
 
 // larger key = larger weight; NaN below everything
 __device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : score_order_key(w); }
@@ -22,143 +26,145 @@ __device__ __forceinline__ uint32_t ld_dsmem(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void st_dsmem(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
-// exclusive sum over the block of two counts
-__device__ __forceinline__ uint2 block_scan2(uint2 v, uint2* warp_sum, uint2* total) {
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  uint2 x = v;
+// sum over the lanes before this one, and over all
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t* total) {
+  const uint32_t lane = threadIdx.x & 31u;
+  uint32_t x = v;
 #pragma unroll
   for (uint32_t o = 1; o < 32; o <<= 1) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, x.x, o), b = __shfl_up_sync(0xffffffffu, x.y, o);
-    if (lane >= o) { x.x += a; x.y += b; }
+    const uint32_t a = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += a;
   }
-  __syncthreads();
-  if (lane == 31) warp_sum[warp] = x;
-  __syncthreads();
-  uint2 w = warp_sum[lane];
-  uint2 y = w;
-#pragma unroll
-  for (uint32_t o = 1; o < 32; o <<= 1) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, y.x, o), b = __shfl_up_sync(0xffffffffu, y.y, o);
-    if (lane >= o) { y.x += a; y.y += b; }
-  }
-  *total = make_uint2(__shfl_sync(0xffffffffu, y.x, 31), __shfl_sync(0xffffffffu, y.y, 31));
-  const uint32_t bx = __shfl_sync(0xffffffffu, y.x - w.x, warp), by = __shfl_sync(0xffffffffu, y.y - w.y, warp);
-  return make_uint2(bx + x.x - v.x, by + x.y - v.y);
+  *total = __shfl_sync(0xffffffffu, x, 31);
+  return x - v;
 }
 
 template <bool IN_REGS>
 __global__ void __launch_bounds__(SEL_T, 1) dg_kv8_select_kernel(const __grid_constant__ EvictParams p, uint32_t ctas) {
-  __shared__ uint32_t hist[BINS];            // this CTA's counts of a digit
-  __shared__ uint32_t sums[BINS];            // the cluster's
-  __shared__ uint2 warp_sum[32];
+  __shared__ uint32_t hist[4][BINS];         // this CTA's counts of a digit
+  __shared__ __align__(16) uint32_t part[4][BINS];         // the cluster's, by pairs of CTAs
+  __shared__ uint32_t warp_gt[32], warp_eq[32];
   __shared__ uint32_t found[2];
-  __shared__ uint32_t totals[2];             // kept and tied tokens of this CTA
+  __shared__ uint32_t ahead_gt, ahead_eq;    // tokens above the cut and at it in the CTAs ahead
   grid_launch_dependents();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = blockIdx.x % ctas, h = blockIdx.x / ctas;
+  hist[tid / BINS][tid % BINS] = 0u;
+  if (tid == 0) ahead_gt = ahead_eq = 0u;
   grid_wait();
-  const uint32_t tid = threadIdx.x, rank = blockIdx.x % ctas, h = blockIdx.x / ctas;
   const float* w = p.w + size_t(h) * p.ld;
   const uint32_t n = p.n_keys - p.n_recent, take = p.n_keep - p.n_recent;
-  const uint32_t seg = (n + ctas - 1) / ctas, per = (seg + SEL_T - 1) / SEL_T;
-  // this thread's run of tokens
-  const uint32_t end_c = (rank + 1) * seg < n ? (rank + 1) * seg : n;
-  uint32_t t0 = rank * seg + tid * per, t1 = t0 + per;
-  if (t0 > end_c) t0 = end_c;
-  if (t1 > end_c) t1 = end_c;
+  // a CTA has `per` times 1,024 tokens, a warp `per` times 32 of them, a lane every 32nd
+  const uint32_t per = ((n + ctas - 1) / ctas + SEL_T - 1) / SEL_T;
+  const uint32_t t0 = (rank * SEL_T + warp * 32u) * per + lane;
   float run[IN_REGS ? RUN : 1];
   if (IN_REGS) {
 #pragma unroll
-    for (uint32_t i = 0; i < RUN; ++i) run[i] = t0 + i < t1 ? __ldg(w + t0 + i) : 0.f;
+    for (uint32_t i = 0; i < RUN; ++i) run[i] = i < per && t0 + i * 32u < n ? __ldg(w + t0 + i * 32u) : 0.f;
   }
-  // f(token, weight) for the tokens of the run, in order
+  // f(token, weight, is there one) for the warp's tokens, in order, by all lanes at once
   auto each = [&](auto f) {
     if (IN_REGS) {
 #pragma unroll
       for (uint32_t i = 0; i < RUN; ++i)
-        if (t0 + i < t1) f(t0 + i, run[i]);
+        if (i < per) f(t0 + i * 32u, run[i], t0 + i * 32u < n);
     } else {
-      for (uint32_t t = t0; t < t1; ++t) f(t, __ldg(w + t));
+#pragma unroll 1
+      for (uint32_t i = 0; i < per; ++i) {
+        const uint32_t t = t0 + i * 32u;
+        f(t, t < n ? __ldg(w + t) : 0.f, t < n);
+      }
     }
   };
-  auto sync_all = [&] {
-    if (ctas > 1) cluster_sync_all(); else __syncthreads();
-  };
+  __syncthreads();
 
-  uint32_t prefix = 0, left = take;          // the digits found so far; tokens to take among those that share them
+  uint32_t cut = 0, left = take;             // the digits found so far; tokens to take among those that share them
   if (take > 0) {
 #pragma unroll 1
-    for (uint32_t pass = 0; pass < 3; ++pass) {
-      const uint32_t shift = pass == 0 ? 21u : pass == 1 ? 10u : 0u, bits = pass == 2 ? 10u : 11u, bins = 1u << bits;
-      hist[tid] = 0u;
-      hist[tid + SEL_T] = 0u;
-      __syncthreads();
-      each([&](uint32_t, float x) {
+    for (uint32_t pass = 0; pass < 4; ++pass) {
+      const uint32_t shift = 24u - 8u * pass, high = pass == 0 ? 0u : 0xffffffffu << (shift + 8u);
+      each([&](uint32_t, float x, bool is) {
         const uint32_t key = weight_key(x);
-        if (pass == 0 || (key >> (shift + bits)) == prefix) atomicAdd(hist + ((key >> shift) & (bins - 1u)), 1u);
+        if (is && ((key ^ cut) & high) == 0u) atomicAdd(&hist[pass][(key >> shift) & (BINS - 1u)], 1u);
       });
-      sync_all();
-      if (ctas > 1) {
-        for (uint32_t i = tid; i < bins / ctas; i += SEL_T) {
-          const uint32_t bin = rank * (bins / ctas) + i;
-          uint32_t s = 0;
-          for (uint32_t r = 0; r < ctas; ++r) s += ld_dsmem(dsmem_addr(smem_u32(hist + bin), r));
-          for (uint32_t r = 0; r < ctas; ++r) st_dsmem(dsmem_addr(smem_u32(sums + bin), r), s);
+      if (ctas > 1) cluster_sync_all(); else __syncthreads();
+      const uint32_t bin = tid % BINS, r = tid / BINS;
+      uint32_t s = 0, ahead = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < MAX_CTAS; i += 4)
+        if (r + i < ctas) {
+          const uint32_t c = ld_dsmem(dsmem_addr(smem_u32(&hist[pass][bin]), r + i));
+          s += c;
+          ahead += r + i < rank ? c : 0u;
         }
-        cluster_sync_all();
-      }
-      // largest digit first: thread i has the bins bins - 1 - 2i and bins - 2 - 2i
-      const uint32_t* src = ctas > 1 ? sums : hist;
-      const uint32_t c0 = 2u * tid < bins ? src[bins - 1u - 2u * tid] : 0u, c1 = 2u * tid < bins ? src[bins - 2u - 2u * tid] : 0u;
-      uint2 total;
-      const uint32_t before = block_scan2(make_uint2(c0 + c1, 0u), warp_sum, &total).x;
-      if (before < left && left <= before + c0 + c1) {
-        const bool in_first = left <= before + c0;
-        found[0] = bins - 1u - 2u * tid - (in_first ? 0u : 1u);
-        found[1] = left - before - (in_first ? 0u : c0);
+      part[r][bin] = s;
+      __syncthreads();
+      if (warp == 0) {
+        // largest digit first: lane i has the bins 255 - 8i down to 248 - 8i
+        uint32_t c[8] = {}, all = 0, total;
+#pragma unroll
+        for (uint32_t r2 = 0; r2 < 4; ++r2)
+#pragma unroll
+          for (uint32_t q = 0; q < 2; ++q) {
+            const uint4 v = *reinterpret_cast<const uint4*>(&part[r2][BINS - 8u - 8u * lane + 4u * q]);
+            c[4 * q] += v.x; c[4 * q + 1] += v.y; c[4 * q + 2] += v.z; c[4 * q + 3] += v.w;
+          }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) all += c[i];
+        uint32_t before = warp_scan(all, &total);
+        if (before < left && left <= before + all) {
+#pragma unroll
+          for (uint32_t i = 8; i-- > 0;) {
+            if (before < left && left <= before + c[i]) {
+              found[0] = BINS - 8u - 8u * lane + i;
+              found[1] = left - before;
+            }
+            before += c[i];
+          }
+        }
       }
       __syncthreads();
-      prefix = (prefix << bits) | found[0];
+      cut |= found[0] << shift;
       left = found[1];
+      if (ctas > 1) {
+        const uint32_t above = __reduce_add_sync(0xffffffffu, bin > found[0] ? ahead : 0u);
+        if (lane == 0 && above != 0u) atomicAdd(&ahead_gt, above);
+        if (pass == 3 && bin == found[0] && ahead != 0u) atomicAdd(&ahead_eq, ahead);
+      }
     }
   }
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   // kept: above the cut, and the first `left` of those at it
   uint32_t gt = 0, eq = 0;
   if (take > 0)
-    each([&](uint32_t, float x) {
-      const uint32_t key = weight_key(x);
-      gt += key > prefix ? 1u : 0u;
-      eq += key == prefix ? 1u : 0u;
+    each([&](uint32_t, float x, bool is) {
+        const uint32_t key = weight_key(x);
+      gt += __popc(__ballot_sync(0xffffffffu, is && key > cut));
+      eq += __popc(__ballot_sync(0xffffffffu, is && key == cut));
     });
-  uint2 total;
-  uint2 at = block_scan2(make_uint2(gt, eq), warp_sum, &total);
-  if (ctas > 1) {
-    if (tid == 0) {
-      totals[0] = total.x;
-      totals[1] = total.y;
-    }
-    cluster_sync_all();
-    for (uint32_t r = 0; r < rank; ++r) {
-      at.x += ld_dsmem(dsmem_addr(smem_u32(&totals[0]), r));
-      at.y += ld_dsmem(dsmem_addr(smem_u32(&totals[1]), r));
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (lane == 0) {
+    warp_gt[warp] = gt;
+    warp_eq[warp] = eq;
   }
+  __syncthreads();
+  uint32_t total;
+  const uint32_t base_gt = warp_scan(warp_gt[lane], &total), base_eq = warp_scan(warp_eq[lane], &total);
+  uint32_t at_gt = ahead_gt + __shfl_sync(0xffffffffu, base_gt, warp), at_eq = ahead_eq + __shfl_sync(0xffffffffu, base_eq, warp);
   int32_t* kept = p.kept + size_t(h) * p.n_keep;
   float* w_out = p.w_out ? p.w_out + size_t(h) * p.ld_out : nullptr;
   if (take > 0)
-    each([&](uint32_t t, float x) {
+    each([&](uint32_t t, float x, bool is) {
       const uint32_t key = weight_key(x);
-      const bool tie = key == prefix;
-      if (key > prefix || (tie && at.y < left)) {
-        const uint32_t o = at.x + (at.y < left ? at.y : left);
+      const uint32_t g = __ballot_sync(0xffffffffu, is && key > cut), q = __ballot_sync(0xffffffffu, is && key == cut);
+      if ((g | q) == 0u) return;
+      const uint32_t ahead = (1u << lane) - 1u;
+      const uint32_t ties = at_eq + __popc(q & ahead);      // those at the cut ahead of this token
+      if (is && key >= cut && (key > cut || ties < left)) {
+        const uint32_t o = at_gt + __popc(g & ahead) + (ties < left ? ties : left);
         kept[o] = int32_t(t);
         if (w_out) w_out[o] = x;
       }
-      at.x += key > prefix ? 1u : 0u;
-      at.y += tie ? 1u : 0u;
+      at_gt += __popc(g);
+      at_eq += __popc(q);
     });
   for (uint32_t i = rank * SEL_T + tid; i < p.n_recent; i += ctas * SEL_T) {
     kept[take + i] = int32_t(n + i);
@@ -226,10 +232,16 @@ __global__ void __launch_bounds__(512) dg_kv8_move_kernel(const __grid_constant_
   if (tid == 0) p.to_exps[(size_t(h) * p.to_blocks + blk) * 2 + (is_k ? 0 : 1)] = e;
 }
 
+cudaError_t configure_evict() {
+  cudaError_t e = cudaFuncSetAttribute(dg_kv8_select_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(dg_kv8_select_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
+}
+
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st) {
-  // CTAs of a head: one up to 4,096 tokens (four each thread), eight from 16,385
+  // CTAs of a head: one up to 4,096 tokens (four each thread), sixteen from 32,769
   uint32_t ctas = 1;
-  while (ctas < 8 && (p.n_keys - p.n_recent) > ctas * 4u * SEL_T) ctas *= 2;
+  while (ctas < MAX_CTAS && (p.n_keys - p.n_recent) > ctas * 4u * SEL_T) ctas *= 2;
   const bool in_regs = p.n_keys - p.n_recent <= ctas * SEL_T * RUN;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas * p.Hkv);
