@@ -54,6 +54,11 @@ static int32_t check_aligned(std::initializer_list<const void*> ps) {
     if (!aligned16(p)) return fail(DG_ERR_ALIGNMENT, "device pointers must be 16-byte aligned");
   return DG_OK;
 }
+// Does [a, a + na) share a byte with [b, b + nb)?  (NULL: no memory.)
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + nb && y < x + na;
+}
 static kv8::Rope make_rope8(const dg_layer_desc& d) {
   kv8::Rope r;
   r.half = d.rotary_dim / 2;
@@ -301,8 +306,20 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
   }
   r = check_aligned({q, k, v, qw, kw, out, q_rot});
   if (r != DG_OK) return r;
-  DG_CUDA(cudaSetDevice(c->device));
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(DG_ERR_ALIGNMENT, "lse must be 4-byte aligned");
   const uint32_t C = d->canvas, G = d->n_q_heads / d->n_kv_heads, D = d->head_dim;
+  {
+    // several CTAs may read a row of q, k or v, and not all at the time when another writes outputs
+    const size_t nq = size_t(batch) * C * d->n_q_heads * D * 2, nk = nq / G, nl = size_t(batch) * C * d->n_q_heads * 4;
+    const struct { const void* p; size_t n; } outs[3] = {{out, nq}, {q_rot, nq}, {lse, nl}}, ins[5] = {{q, nq}, {k, nk}, {v, nk}, {qw, D * 2u}, {kw, D * 2u}};
+    for (int i = 0; i < 3; ++i) {
+      for (const auto& x : ins)
+        if (overlap(outs[i].p, outs[i].n, x.p, x.n)) return fail(DG_ERR_INVALID_ARG, "an output overlaps an input");
+      for (int j = 0; j < i; ++j)
+        if (overlap(outs[i].p, outs[i].n, outs[j].p, outs[j].n)) return fail(DG_ERR_INVALID_ARG, "two outputs overlap");
+    }
+  }
+  DG_CUDA(cudaSetDevice(c->device));
   const uint32_t MT = (C * G + BLK - 1) / BLK, n_ctiles = k ? (C + BLK - 1) / BLK : 0, KU = D / 256;
   const bool token = C * G <= kv8::TOKEN_ROWS && C <= kv8::TOKEN_CANVAS;
   const size_t q_elems = size_t(C) * d->n_q_heads * D, kv_elems = size_t(C) * d->n_kv_heads * D;
@@ -438,6 +455,11 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   if (r != DG_OK) return r;
   if ((reinterpret_cast<uintptr_t>(lse) & 3u) || (reinterpret_cast<uintptr_t>(weights) & 3u))
     return fail(DG_ERR_ALIGNMENT, "lse and weights must be 4-byte aligned");
+  {
+    const size_t rows = size_t(d->canvas) * d->n_q_heads, n_w = ((d->n_kv_heads - 1) * ld + n_keys) * 4;
+    if (overlap(weights, n_w, q_rot, rows * d->head_dim * 2) || overlap(weights, n_w, lse, rows * 4))
+      return fail(DG_ERR_INVALID_ARG, "weights overlaps an input");
+  }
   c->last_launches = 0;
   if (n_keys == 0) return DG_OK;
   DG_CUDA(cudaSetDevice(c->device));
@@ -468,8 +490,10 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   p.ld = ld;
   p.decay = decay;
   p.status = c->d_status;
-  // One CTA a run of keys where the runs are a whole number of waves or few steps long; else an even cut of all steps, runs shared
-  // at the cuts: 2 steps for what a second launch costs, 2 for what a run or a CTA costs beside its steps (1.2 us each).
+  // One CTA a run of keys, or an even cut of all steps with the runs shared at the cuts and a second launch for the sums: by
+  // steps a CTA (1.3 us and less), 2 for what a run costs beside its steps, 4 for the launch.  us by runs / cut evenly, a canvas
+  // of 256 over 2 KV heads of head_dim 256: 2,000 keys 30.7 / 22.1, 8,191 33.4 / 27.6, 19,200 59.2 / 43.0, 32,768 60.4 / 61.8,
+  // 45,000 86.8 / 80.0; a canvas of 64, head_dim 512: 8,191 15.6 / 20.7, 19,200 36.7 / 30.8.
   const uint32_t sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u, kt = 512 / D, blocks = (n_keys + BLK - 1) / BLK;
   {
     MaskParams mk = make_mask(*d, n_keys, 0, n_keys, 0);
@@ -507,10 +531,9 @@ extern "C" int32_t dg_kv8_evict(dg_ctx* c, dg_kv8* from, uint32_t n_keys, const 
   if (ld < n_keys || (weights_out && ld_out < n_keep)) return fail(DG_ERR_INVALID_ARG, "a row of weights is shorter than its tokens");
   for (const void* p : {static_cast<const void*>(weights), static_cast<const void*>(kept), static_cast<const void*>(weights_out)})
     if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(DG_ERR_ALIGNMENT, "weights and kept must be 4-byte aligned");
-  if (weights_out) {
-    const float *a0 = weights, *a1 = weights + (from->Hkv - 1) * ld + n_keys, *b0 = weights_out, *b1 = weights_out + (from->Hkv - 1) * ld_out + n_keep;
-    if (a0 < b1 && b0 < a1) return fail(DG_ERR_INVALID_ARG, "weights_out overlaps weights");
-  }
+  const size_t heads = from->Hkv - 1, n_w = (heads * ld + n_keys) * 4, n_o = (heads * ld_out + n_keep) * 4, n_i = (heads + 1) * n_keep * 4;
+  if (overlap(weights, n_w, weights_out, n_o)) return fail(DG_ERR_INVALID_ARG, "weights_out overlaps weights");
+  if (overlap(kept, n_i, weights, n_w) || overlap(kept, n_i, weights_out, n_o)) return fail(DG_ERR_INVALID_ARG, "kept overlaps weights");
   DG_CUDA(cudaSetDevice(c->device));
   kv8::EvictParams p = {};
   p.w = weights;

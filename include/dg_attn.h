@@ -348,7 +348,7 @@ int32_t dg_kv8_read(dg_kv8* kv, void* k_out, void* v_out, uint64_t slot0, uint64
  * zeros.  pos[b] (host array; NULL: n_keys) is the position of canvas row 0.  A window counts positions and needs
  * pos[b] = n_keys[b].  The same cache may serve several canvases.  out: bf16 [batch][C][Hq][D]; lse (or NULL): fp32
  * [batch][C][Hq], ln of the sum of e^score over what a row sees, -inf where it sees nothing; q_rot (or NULL): the normed
- * and rotated queries, bf16 [batch][C][Hq][D].                                                                          */
+ * and rotated queries, bf16 [batch][C][Hq][D].  Outputs overlap neither inputs nor each other.                          */
 int32_t dg_kv8_denoise(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* const* kv, const uint32_t* n_keys, const uint64_t* pos,
                        uint32_t batch, const void* q, const void* k, const void* v, const void* qw, const void* kw, void* out,
                        float* lse, void* q_rot);

@@ -196,7 +196,8 @@ CASES = [
     (dict(n_q_heads=6, n_kv_heads=2), 100, 500, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 300, dict(mask_mode=CAUSAL)),
     (dict(n_q_heads=3, n_kv_heads=3), 7, 200, {}), (dict(n_q_heads=40, n_kv_heads=1), 33, 200, {}),
     ({**GLOBAL, "rotary_dim": 64}, 20, 300, {}), ({**GLOBAL, "rotary_dim": 0}, 20, 300, {}), ({**GLOBAL, "softmax_scale": 1.0}, 40, 900, {}),
-    ({**FULL, "rotary_dim": 512, "rope_pairing": capi.ROPE_SPLIT_HALF}, 20, 300, {}),
+    (SLIDING, 8, 400, {}), (SLIDING, 9, 400, {}), (FULL, 2, 400, dict(mask_mode=CAUSAL)), (dict(n_q_heads=4, n_kv_heads=4), 8, 400, dict(mask_mode=CAUSAL)),
+    (dict(n_q_heads=4, n_kv_heads=4), 16, 400, {}), ({**FULL, "rotary_dim": 512, "rope_pairing": capi.ROPE_SPLIT_HALF}, 20, 300, {}),
 ]
 
 
@@ -216,6 +217,45 @@ def test_attention(ctx, geo, canvas, n, more, splits):
     assert torch.equal(q_rot[0].double(), qr)
     assert torch.equal(out, again) and ctx.device_status()[0] == 0
     kv.close()
+
+
+@pytest.mark.parametrize("geo,canvas", [(GLOBAL, 1), (FULL, 1), (GLOBAL, 64), (FULL, 64)])
+@pytest.mark.parametrize("splits", [9, 17, 32])
+def test_many_splits(ctx, geo, canvas, splits):
+    layer = AttnLayer(canvas=canvas, **geo)
+    kv, hk, hv = filled(ctx, layer, 4200, 2)
+    q, k, v, qw, kw = step_inputs(layer, 1, 6)
+    ctx.set_splits(splits)
+    try:
+        out, lse = CanvasAttention(ctx, layer).denoise_kv8([kv], [4200], q, k, v, qw, kw, with_lse=True)
+    finally:
+        ctx.set_splits(0)
+    check_step(layer, out[0], lse[0], q[0], k[0], v[0], qw, kw, 4200, 4200, hk, hv)
+    kv.close()
+
+
+@pytest.mark.parametrize("canvas", [1, 100])
+def test_two_contexts_at_once(ctx, canvas):
+    """Two contexts, each with its own stream and scratch, over one cache at the same time."""
+    layer = AttnLayer(canvas=canvas, **GLOBAL)
+    kv, hk, hv = filled(ctx, layer, 9000, 4)
+    ctx.synchronize()
+    owns = [Context(0, make_current=False) for _ in range(2)]
+    steps = [step_inputs(layer, 1, 20 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, own in enumerate(owns):
+            with torch.cuda.stream(own.torch_stream):
+                got[i].append(CanvasAttention(own, layer).denoise_kv8([kv], [9000], *steps[i], with_lse=True))
+    for own in owns:
+        own.synchronize()
+    for i, (q, k, v, qw, kw) in enumerate(steps):
+        check_step(layer, got[i][0][0][0], got[i][0][1][0], q[0], k[0], v[0], qw, kw, 9000, 9000, hk, hv)
+        assert all(torch.equal(out, got[i][0][0]) and torch.equal(lse, got[i][0][1]) for out, lse in got[i])
+    kv.close()
+    for own in owns:
+        own.close()
 
 
 @pytest.mark.parametrize("geo", [GLOBAL, FULL])
@@ -333,7 +373,8 @@ def test_a_strong_first_token_loses_none_of_the_weak_ones(ctx, geo):
     (GLOBAL, 1, 1, {}), (GLOBAL, 1, 129, {}), (SLIDING, 1, 4000, {}), (GLOBAL, 256, 1000, {}), (SLIDING, 77, 1300, {}),
     (SLIDING, 256, 1500, dict(window=300, mask_mode=PER_ROW)), (SLIDING, 256, 1500, dict(window=300, mask_mode=UNIFORM)),
     (SLIDING, 200, 900, dict(window=100, mask_mode=CAUSAL)), (GLOBAL, 200, 900, dict(mask_mode=CAUSAL)), (FULL, 1, 300, {}), (FULL, 256, 700, {}),
-    (FULL, 90, 400, dict(window=64, mask_mode=PER_ROW)), (dict(n_q_heads=6, n_kv_heads=2), 50, 300, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 9000, {})])
+    (FULL, 90, 400, dict(window=64, mask_mode=PER_ROW)), (SLIDING, 20, 9000, dict(window=300, mask_mode=PER_ROW)), (GLOBAL, 256, 9001, {}),
+    (FULL, 1, 5000, dict(window=2, mask_mode=CAUSAL)), (FULL, 256, 5000, {}), (dict(n_q_heads=6, n_kv_heads=2), 50, 300, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 9000, {})])
 @pytest.mark.parametrize("decay", [0.0, 1.0, 0.25])
 def test_key_weights(ctx, geo, canvas, n, more, decay):
     layer = AttnLayer(canvas=canvas, **{**geo, **more})
@@ -371,7 +412,8 @@ def test_key_weights_add_up_to_the_rows(ctx):
 # ------------------------------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("geo,n,n_keep,n_recent", [
     (SLIDING, 1, 1, 0), (GLOBAL, 1, 1, 1), (GLOBAL, 300, 100, 0), (GLOBAL, 300, 300, 0), (GLOBAL, 300, 300, 300), (GLOBAL, 300, 17, 17),
-    (SLIDING, 5003, 1250, 257), (FULL, 1000, 129, 1), (FULL, 2049, 2048, 3), (GLOBAL, 8193, 8192, 0), (GLOBAL, 150000, 4097, 100)])
+    (SLIDING, 5003, 1250, 257), (FULL, 1000, 129, 1), (FULL, 2049, 2048, 3), (GLOBAL, 8193, 8192, 0), (GLOBAL, 20001, 5000, 1),
+    (GLOBAL, 150000, 4097, 100), (GLOBAL, 270000, 300, 7)])
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
 def test_evict(ctx, geo, n, n_keep, n_recent, kind):
     layer = AttnLayer(**geo)
@@ -541,7 +583,15 @@ def test_refusals(ctx):
     assert denoise(pos=2 ** 31 - 3) == capi.DG_ERR_CAPACITY
     assert denoise(desc=bad(window=5, mask_mode=UNIFORM), pos=101) == capi.DG_ERR_INVALID_ARG
     assert denoise(desc=bad(canvas=257)) == capi.DG_ERR_UNSUPPORTED
-    assert b"pos = n_keys" in lib.dg_last_error_message() or True
+
+    def outputs(out_=p(out), lse_=None, q_rot_=None):
+        return lib.dg_kv8_denoise(ctx.h, C.byref(d), (C.c_void_p * 1)(kv.h), (C.c_uint32 * 1)(100), None, 1, p(q), p(k), p(v), p(qw), p(kw),
+                                  out_, lse_, q_rot_)
+
+    assert outputs(out_=p(q)) == capi.DG_ERR_INVALID_ARG and outputs(q_rot_=p(q)) == capi.DG_ERR_INVALID_ARG
+    assert outputs(out_=C.c_void_p(k.data_ptr() + 16)) == capi.DG_ERR_INVALID_ARG and outputs(q_rot_=p(out)) == capi.DG_ERR_INVALID_ARG
+    assert outputs(lse_=C.c_void_p(out.data_ptr() + 64)) == capi.DG_ERR_INVALID_ARG
+    assert outputs(lse_=C.c_void_p(lse.data_ptr() + 2)) == capi.DG_ERR_ALIGNMENT
     k2 = randn(1, 30, 2, 256)
     assert lib.dg_kv8_append(ctx.h, C.byref(d), kv.h, 100, 100, 29, p(k2), p(k2), None) == capi.DG_ERR_CAPACITY
     assert lib.dg_kv8_append(ctx.h, C.byref(d), kv.h, 100, 2 ** 31, 1, p(k2), p(k2), None) == capi.DG_ERR_CAPACITY
@@ -554,6 +604,7 @@ def test_refusals(ctx):
 
     weigh = lambda n=100, ld=128, decay=1.0: lib.dg_kv8_key_weights(ctx.h, C.byref(d), kv.h, n, p(q), p(lse), p(w), ld, decay)
     assert weigh(n=129) == capi.DG_ERR_CAPACITY and weigh(ld=99) == capi.DG_ERR_INVALID_ARG
+    assert lib.dg_kv8_key_weights(ctx.h, C.byref(d), kv.h, 100, p(q), p(lse), p(lse), 128, 1.0) == capi.DG_ERR_INVALID_ARG
     assert weigh(decay=-1.0) == capi.DG_ERR_INVALID_ARG and weigh(decay=math.nan) == capi.DG_ERR_INVALID_ARG and weigh(n=0) == capi.DG_OK
     to = KvCache8(ctx, layer, 50)
 
@@ -563,7 +614,7 @@ def test_refusals(ctx):
     assert evict(dst=kv) == capi.DG_ERR_INVALID_ARG and evict(src=other) == capi.DG_ERR_INVALID_ARG
     assert evict(keep=0) == capi.DG_ERR_INVALID_ARG and evict(keep=101) == capi.DG_ERR_INVALID_ARG and evict(recent=51) == capi.DG_ERR_INVALID_ARG
     assert evict(keep=129, n=128) == capi.DG_ERR_CAPACITY and evict(n=129) == capi.DG_ERR_CAPACITY and evict(ld=99) == capi.DG_ERR_INVALID_ARG
-    assert evict(w_out=p(w)) == capi.DG_ERR_INVALID_ARG
+    assert evict(w_out=p(w)) == capi.DG_ERR_INVALID_ARG and evict(w_out=p(kept)) == capi.DG_ERR_INVALID_ARG
     ctx.synchronize()
     for c in (kv, other, to):
         c.close()
