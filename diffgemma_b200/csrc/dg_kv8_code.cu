@@ -17,13 +17,16 @@ struct PosList {
 // A warp takes one row.  Canvas K and V: the rows of one (head, tile, K or V) share a scale; they lie in `slots` neighbouring
 // warps (up to 16 canvas tokens) or in the CTAs of a cluster, 16 tokens each, whose maxima meet over distributed shared memory.
 // Queries: a CTA for each canvas token, all heads (the angles are computed once for all of them).
+// A step's rows of 256 tokens: 14 us (8 KV heads of 256 dims), 13.5 (2 of 512), most of it one chain - launch, loads, angles,
+// norm, rotation, the cluster's maxima, stores; two or three tokens a CTA, which make one wave of two, take as long.
 struct RowsPlan {
   uint32_t slots, cluster;             // warps of a scale group in a CTA; CTAs of one (16 slots)
   uint32_t canvas_ctas, per_seq;       // CTAs of canvas rows; of them, of a sequence
   uint32_t heads;                      // KV heads that a CTA of 16 slots takes one after the other
   uint32_t q_tokens, q_ctas;           // query CTAs of a sequence, of all
 };
-constexpr uint32_t ROW_HEADS = 4;
+// heads that a CTA of 16 slots holds in registers
+__host__ __device__ constexpr uint32_t row_heads(int nj) { return nj == 1 ? 4u : 2u; }
 
 // One row of canvas K or V: normed, rotated, rounded, what is not finite as zero.  Returns its largest magnitude.
 template <int NJ>
@@ -73,6 +76,7 @@ template <int NJ>
 __global__ void __launch_bounds__(CT, NJ == 1 ? 2 : 1) dg_kv8_rows_kernel(const __grid_constant__ QueryParams q, const __grid_constant__ CodeParams p,
                                                                          const __grid_constant__ PosList pos, const __grid_constant__ RowsPlan plan) {
   extern __shared__ __align__(16) uint8_t smem[];
+  constexpr uint32_t ROW_HEADS = row_heads(NJ);
   __shared__ float red[ROW_HEADS][16];
   grid_launch_dependents();
   grid_wait();
@@ -449,7 +453,8 @@ cudaError_t launch_rows(const QueryParams& q, const CodeParams& p, const uint64_
     } else {
       const uint32_t tokens = p.n < BLK ? p.n : BLK;
       while (plan.cluster * 16u < tokens) plan.cluster *= 2u;
-      plan.heads = q.rows.Hkv < ROW_HEADS ? q.rows.Hkv : ROW_HEADS;
+      const uint32_t most = row_heads(int(q.rows.D / 256u));
+      plan.heads = q.rows.Hkv < most ? q.rows.Hkv : most;
       plan.per_seq = (q.rows.Hkv + plan.heads - 1u) / plan.heads * p.n_ctiles * 2u;
       plan.canvas_ctas = n_seq * plan.per_seq * plan.cluster;
     }

@@ -70,7 +70,18 @@ __device__ __forceinline__ void row_to_bf16(const uint4 (&raw)[NJ], const __nv_b
       }
     }
   }
-  if (tab != nullptr && rope.half != 0) {
+  if (tab != nullptr && NJ == 2 && rope.dist == 256u) {        // a pair lies in one lane
+    const uint32_t hc = rope.half >> 3;
+    if (lane < hc) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const typename Pair<T>::type cs = tab[i * hc + lane];
+        const T a = x[0][i], b = x[NJ - 1][i];
+        x[0][i] = fma(b, -cs.y, a * cs.x);
+        x[NJ - 1][i] = fma(a, cs.y, b * cs.x);
+      }
+    }
+  } else if (tab != nullptr && rope.half != 0) {
     // chunks of 8 elements: chunk c < half / 8 pairs with chunk c + dist / 8
     const uint32_t hc = rope.half >> 3, dc = rope.dist >> 3;
     T y[NJ][8];
