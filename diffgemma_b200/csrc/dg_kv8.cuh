@@ -134,6 +134,33 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
       : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// the same by the leader of a CTA pair, over both CTAs' operands
+__device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// all prior MMAs of this thread arrive once on the barrier at this offset of both CTAs of the pair
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3)) : "memory");
+}
 // contiguous copy global -> this CTA's shared memory, counted on a local barrier; both 16-byte aligned, bytes a multiple of 16
 __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst),
@@ -142,12 +169,15 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
 }
 // mbar_wait with its clock and the abort flag looked at every 64th poll only: a waiting warp shares its scheduler with warps that
 // compute, and a poll alone is a third of the instructions.
+// CLUSTER: arrivals may come from the pair's other CTA.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
+  auto there = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (there()) return true;
   const long long t0 = clock64();
 #pragma unroll 1
   for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (there()) return true;
     if ((it & 63u) == 0u) {
       if (*abort_flag) return false;
       if (clock64() - t0 > DG_WAIT_LIMIT_CYCLES) {
@@ -230,8 +260,8 @@ struct AttnParams8 {
   uint32_t n_ctiles;
   __nv_bfloat16* out;          // [seq][C][Hq][D]
   float* lse;                  // [seq][C][Hq] or null
-  float* ws_o;                 // split partials [CTA][128][256]
-  float2* ws_ml;               // [CTA][128]
+  float* ws_o;                 // split partials [slot][128][256], slot: sequence's first CTA + ((split * Hkv + head) * MT + row tile) * D / 256 + half
+  float2* ws_ml;               // [slot][128]
   DevStatus* status;
 };
 
@@ -340,7 +370,7 @@ cudaError_t launch_append(const CodeParams& p, cudaStream_t st);
 cudaError_t launch_read(const ReadParams& p, cudaStream_t st);
 cudaError_t launch_token(const TokenParams& p, uint32_t D, uint32_t n_ctas, cudaStream_t st);
 cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_t st);
-cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st);
+cudaError_t launch_attention(const AttnParams8& p, bool pair, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st);
 cudaError_t launch_weights(const WeightParams& p, uint32_t D, uint32_t ctas, cudaStream_t st);
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st);
 

@@ -436,7 +436,7 @@ extern "C" int32_t dg_kv8_denoise(dg_ctx* c, const dg_layer_desc* d, dg_kv8* con
     p.c_v = ws + l.cv;
     p.c_exps = reinterpret_cast<const int2*>(cp.exps);
     DG_CUDA(kv8::launch_rows(qp, cp, at, n, c->stream));
-    DG_CUDA(kv8::launch_attention(p, ctas, splits, c->stream));
+    DG_CUDA(kv8::launch_attention(p, D == 512 && MT % 2 == 0, ctas, splits, c->stream));
     c->last_launches += splits > 1 ? 3 : 2;
   }
   return DG_OK;

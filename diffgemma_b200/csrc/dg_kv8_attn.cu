@@ -12,8 +12,14 @@
 // e5m2 reaches 2^-16, 2^-21 of the largest weight: a strong first token beside 10^5 weak ones loses none of them.
 // Tiles of the canvas come as two terms as well (K = k1 + k2, V = v1 + v2: the rows' bf16 values) and pass twice.
 //
-// Per 128 keys and 256 dims: 2,048 cycles of MMA, 64 KB from L2 / HBM, 256 KB of shared-memory traffic (Q 128, K 64 as
-// operands read twice, V 64 likewise ... half of what bf16 operands move), 16,384 exponentials (1,024 cycles).
+// Per 128 keys, 256 dims: 2,048 cycles of MMA, 64 KB from L2 / HBM, 16,384 exponentials (1,024 cycles), and 256 KB through
+// shared memory (S: 4 KB of Q and 4 KB of K for each MMA of 64 cycles; PV 64 KB; the copies 64 KB), which at 128 bytes a cycle
+// takes as long as the MMAs.  Measured: 2,600 cycles, the rest is the way from scores to weights and the waits between
+// (32,768 keys of 2 KV heads, 256 rows: 122 us).
+// head_dim 512: 3,072 cycles of MMA and 416 KB (3,328 cycles) a tile, 3,820 measured.  There two row tiles make a pair of CTAs
+// (cta_group::2, M = 256): each brings half of K's tokens and half of V's dims, so that copies and B operands halve (272 KB).
+// 256 rows over 2 KV heads, us alone / in pairs: 2,000 keys 47.6 / 46.7, 8,000 98.5 / 93.3, 32,000 313.6 / 285.9; a canvas
+// of 64, 32,000 keys 91.1 / 88.9.  head_dim 256 gains nothing (122 / 128: its tiles are too short to hide the other CTA's word).
 #include "dg_kv8.cuh"
 
 namespace dg {
@@ -21,15 +27,18 @@ namespace kv8 {
 
 constexpr uint32_t T_S = 0, T_O = 256;          // tensor memory: two S buffers of 128 columns, O
 constexpr float LAG = 3.0f;                     // 2^(LAG + LIFT) = 256 <= 448
-constexpr uint32_t SM_WARPS = 16, W_K = 16, W_V = 17, W_MMA = 18, THREADS = 19 * 32;
+constexpr uint32_t SM_WARPS = 16, W_K = 16, W_V = 17, W_MMA = 18, W_PASS = 19;   // W_PASS: CTA pairs only
 // B_P_FULL of a tile counts its softmax warps and the bytes of its first V unit; B_V2_FULL those of a canvas tile's second
-enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V2_FULL = 8, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 13, N_BARS = 15 };
+enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 6, B_V2_FULL = 10, B_V_EMPTY = 11, B_S_FULL = 13, B_P_FULL = 15, B_V_OWN = 17, N_BARS = 19 };
 
-template <uint32_t D> struct Cfg {
+template <uint32_t D, bool PAIR> struct Cfg {
+  static constexpr uint32_t THREADS = (PAIR ? W_PASS + 1 : W_PASS) * 32;
   static constexpr uint32_t KU = D / 256;                       // K units of a tile (32 KB each)
-  static constexpr uint32_t NK = D == 256 ? 3 : 2, NV = D == 256 ? 2 : 1;   // stages
+  static constexpr uint32_t NK = PAIR ? 4 : D == 256 ? 3 : 2, NV = PAIR || D == 256 ? 2 : 1;   // stages
+  static_assert(!PAIR || D == 512, "pairs: see launch_attention");
+  static constexpr uint32_t HAVE = PAIR ? UNIT / 2 : UNIT;      // bytes of a unit in this CTA
   static constexpr uint32_t Q_BYTES = 2 * BLK * D;
-  static constexpr uint32_t O_K = Q_BYTES, O_V = O_K + NK * UNIT, O_X = O_V + NV * UNIT;
+  static constexpr uint32_t O_K = Q_BYTES, O_V = O_K + NK * HAVE, O_X = O_V + NV * HAVE;
   static constexpr uint32_t X_BYTES = 4 * BLK * 4;              // row maxima of a row's four threads
   static constexpr uint32_t O_BAR = O_X + X_BYTES, SMEM = O_BAR + N_BARS * 8 + 16;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
@@ -68,9 +77,9 @@ __device__ __forceinline__ void hide32(uint32_t (&s)[32], uint32_t lo, uint32_t 
     if (!((seen >> e) & 1u)) s[e] = 0xff800000u;
 }
 
-template <uint32_t D>
-__global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_constant__ AttnParams8 p) {
-  typedef Cfg<D> cf;
+template <uint32_t D, bool PAIR>
+__global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(const __grid_constant__ AttnParams8 p) {
+  typedef Cfg<D, PAIR> cf;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s0 = smem_u32(smem);
   volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + cf::O_BAR + N_BARS * 8);   // {abort, tmem}
@@ -91,15 +100,19 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     if (b + step < p.n_seq && p.seq[b + step].first_cta <= blockIdx.x) b += step;
   const Seq& sq = p.seq[b];
   uint32_t item = blockIdx.x - sq.first_cta;
+  const uint32_t rank = PAIR ? item & 1u : 0u;                 // in the pair; the leader is 0
+  if (PAIR) item >>= 1;
   const uint32_t z = item % cf::KU;
   item /= cf::KU;
-  const uint32_t mt = item % p.MT;
-  item /= p.MT;
+  const uint32_t row_tiles = PAIR ? p.MT / 2u : p.MT;
+  const uint32_t mt0 = PAIR ? item % row_tiles * 2u : item % row_tiles, mt = mt0 + rank;
+  item /= row_tiles;
   const uint32_t kvh = item % p.Hkv, split = item / p.Hkv;
+  const uint32_t slot = sq.first_cta + ((split * p.Hkv + kvh) * p.MT + mt) * cf::KU + z;
   const MaskParams mk = seq_mask(p, sq.n_keys);
   const uint32_t rows_per_head = p.C * p.G;
-  const uint32_t R_last = (mt + 1) * BLK < rows_per_head ? (mt + 1) * BLK - 1 : rows_per_head - 1;
-  const Tiles ts = tiles_of(mk, mt * BLK / p.G, R_last / p.G);
+  const uint32_t R_end = (mt0 + (PAIR ? 2u : 1u)) * BLK, R_last = R_end < rows_per_head ? R_end - 1 : rows_per_head - 1;
+  const Tiles ts = tiles_of(mk, mt0 * BLK / p.G, R_last / p.G);   // a pair's two row tiles pass over the same keys
   const uint32_t n0 = split_cut(ts, split, sq.n_splits), n1 = split_cut(ts, split + 1, sq.n_splits);
   const uint32_t n_local = n1 - n0;
   const uint32_t n_cached = ts.nA > n0 ? (ts.nA - n0 < n_local ? ts.nA - n0 : n_local) : 0u;   // cached tiles come first
@@ -115,16 +128,27 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
 
   if (tid == 0) {
     ctl[0] = 0u;
-    for (uint32_t i = 0; i < N_BARS; ++i)
-      mbar_init(bar(i), i >= B_P_FULL ? SM_WARPS + 1u : 1u);
+    // the leader's barriers count the other CTA's share as well: its softmax warps, and a word that its operands are there
+    const uint32_t both = PAIR && rank == 0u ? 2u : 1u;
+    for (uint32_t i = 0; i < N_BARS; ++i) {
+      uint32_t count = 1u;
+      if (i == B_Q || i == B_V2_FULL || (i >= B_K_FULL && i < B_K_EMPTY)) count = both;
+      if (i == B_P_FULL || i == B_P_FULL + 1) count = rank != 0u ? SM_WARPS : both * (SM_WARPS + 1u);
+      mbar_init(bar(i), count);
+    }
     fence_mbar_init();
   }
   if (warp == W_MMA) {
-    tmem_alloc(smem_u32(const_cast<uint32_t*>(&ctl[1])), 512);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(&ctl[1])), 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(const_cast<uint32_t*>(&ctl[1])), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl[1];
   grid_wait();
@@ -149,6 +173,12 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     const int2* ep = sq.exps + size_t(kvh) * sq.blocks + ts.a0 + n0;
     const int2* ec = p.c_exps + head_tile + (n0 > ts.nA ? n0 - ts.nA : 0u);
     uint32_t lo = rv.lo, hi = mk.pre_hi, k0 = (ts.a0 + n0) * BLK + part * 32u, stage = 0, phase = 0;
+    // this warp's rows of P are there: for the MMA warp, and for the warps that wait for its reads
+    auto p_ready = [&](uint32_t sb) {
+      if (lane != 0) return;
+      mbar_arrive(bar(B_P_FULL + sb));
+      if (PAIR && rank != 0u) mbar_arrive_remote(dsmem_addr(bar(B_P_FULL + sb), 0u));
+    };
     int2 ex = make_int2(0, 0);
     if (n_local > 0) ex = n_cached > 0 ? *ep : *ec;
     if (n_cached == 0) ep = ec;
@@ -177,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       if (!__all_sync(0xffffffffu, there)) break;
       if (!warp_on) {
         // rows behind the last one: their P stays whatever it is, no row of the output reads it
-        if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+        p_ready(sb);
         continue;
       }
       tc_fence_after();
@@ -224,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_P_FULL + sb));
+      p_ready(sb);
       float a, d;
       unpack_f32x2(add_f32x2(ls[0], ls[1]), a, d);
       l_run = fmaf(a + d, pow2i(-ev), l_run);
@@ -244,8 +274,14 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
         for (uint32_t i = 0; i < units; ++i, ++u) {
           const uint32_t st = u % cf::NK;
           if (u >= cf::NK && !bar_wait(bar(B_K_EMPTY + st), (u / cf::NK - 1u) & 1u, abort_flag)) { ok = false; break; }
-          mbar_expect_tx(bar(B_K_FULL + st), UNIT);
-          bulk_load(s0 + cf::O_K + st * UNIT, src + size_t(i) * UNIT, UNIT, bar(B_K_FULL + st));
+          mbar_expect_tx(bar(B_K_FULL + st), cf::HAVE);
+          const uint32_t dst = s0 + cf::O_K + st * cf::HAVE;
+          if (PAIR) {   // 64 of the 128 tokens
+            for (uint32_t sl = 0; sl < 2; ++sl)
+              bulk_load(dst + sl * (SLAB / 2u), src + size_t(i) * UNIT + sl * SLAB + rank * (SLAB / 2u), SLAB / 2u, bar(B_K_FULL + st));
+          } else {
+            bulk_load(dst, src + size_t(i) * UNIT, UNIT, bar(B_K_FULL + st));
+          }
         }
       }
     }
@@ -256,17 +292,38 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       for (uint32_t t = n0; ok && t < n1; ++t) {
         const bool cached = t < ts.nA;
         const uint8_t* src = (cached ? sq.v + (size_t(kvh) * sq.blocks + ts.a0 + t) * BLK * D
-                                     : p.c_v + size_t(head_tile + t - ts.nA) * 2u * BLK * D) + size_t(z) * UNIT;
+                                     : p.c_v + size_t(head_tile + t - ts.nA) * 2u * BLK * D) + size_t(z) * UNIT + rank * SLAB;   // (a pair's CTAs: 128 of the 256 dims each)
         for (uint32_t i = 0; i < (cached ? 1u : 2u); ++i, ++u) {
           const uint32_t st = u % cf::NV;
           if (u >= cf::NV && !bar_wait(bar(B_V_EMPTY + st), (u / cf::NV - 1u) & 1u, abort_flag)) { ok = false; break; }
-          const uint32_t full = bar(i == 0 ? B_P_FULL + ((t - n0) & 1u) : B_V2_FULL);
-          mbar_expect_tx(full, UNIT);
-          bulk_load(s0 + cf::O_V + st * UNIT, src + size_t(i) * BLK * D, UNIT, full);
+          const uint32_t full = bar(i == 0 ? (rank == 0u ? B_P_FULL : B_V_OWN) + ((t - n0) & 1u) : B_V2_FULL);
+          mbar_expect_tx(full, cf::HAVE);
+          bulk_load(s0 + cf::O_V + st * cf::HAVE, src + size_t(i) * BLK * D, cf::HAVE, full);
         }
       }
     }
-  } else if (n_local > 0) {
+  } else if (PAIR && rank != 0u) {
+    // Tells the leader what has come here: Q and K one warp, V the other (an arrival at cluster scope takes some 700 cycles; one
+    // warp for both was late for the next tile).  The bytes came through the async proxy and are read through it.
+    auto pass_on = [&](uint32_t own, uint32_t parity, uint32_t lead) -> bool {
+      if (!bar_wait(bar(own), parity, abort_flag)) return false;
+      mbar_arrive_cluster(dsmem_addr(bar(lead), 0u));
+      return true;
+    };
+    if (lane == 0 && n_local > 0) {
+      if (warp == W_MMA) {
+        const uint32_t units = (n_cached + 2u * (n_local - n_cached)) * cf::KU;
+        bool ok = pass_on(B_Q, 0u, B_Q);
+        for (uint32_t u = 0; ok && u < units; ++u) ok = pass_on(B_K_FULL + u % cf::NK, (u / cf::NK) & 1u, B_K_FULL + u % cf::NK);
+      } else {
+        bool ok = true;
+        for (uint32_t n = 0; ok && n < n_local; ++n) {
+          ok = pass_on(B_V_OWN + (n & 1u), (n >> 1) & 1u, B_P_FULL + (n & 1u));
+          if (ok && n >= n_cached) ok = pass_on(B_V2_FULL, (n - n_cached) & 1u, B_V2_FULL);
+        }
+      }
+    }
+  } else if (warp == W_MMA && n_local > 0) {
     // The whole warp runs the loop, one elected lane issues.  A wait costs this warp some 150 cycles in which it issues nothing;
     // one before each group of 1,024 cycles of MMAs and one commit behind it keep the tensor pipe full (2,054 cycles for the 24
     // MMAs of a 256-wide tile; two waits and two commits: 2,360), so V's bytes are counted where P's arrivals are and a K
@@ -274,27 +331,30 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     // below 256 KB: the address field cannot carry).
     constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);           // 8-row groups 1024 apart, version 1, 128-byte swizzle
     auto desc = [](uint32_t lo) { return (uint64_t(HI) << 32) | uint64_t(lo); };
-    constexpr uint32_t IDESC = idesc_f8(128, 128, 0, 0), IDESC_P1 = idesc_f8(128, 256, 0, 1), IDESC_P2 = idesc_f8(128, 256, 1, 1);
+    constexpr uint32_t M = PAIR ? 256 : 128;
+    constexpr uint32_t IDESC = idesc_f8(M, 128, 0, 0), IDESC_P1 = idesc_f8(M, 256, 0, 1), IDESC_P2 = idesc_f8(M, 256, 1, 1);
+    auto commit = [&](uint32_t b) { if (PAIR) commit_both(bar(b)); else umma_commit(bar(b)); };
     const uint32_t dq = ((s0 >> 4) & 0x3fffu) | (1u << 16), dk = (((s0 + cf::O_K) >> 4) & 0x3fffu) | (1u << 16);
     const uint32_t dv = (((s0 + cf::O_V) >> 4) & 0x3fffu) | ((SLAB >> 4) << 16);   // MN-major: 128-column chunks SLAB apart
-    bool ok = __all_sync(0xffffffffu, bar_wait(bar(B_Q), 0u, abort_flag));
+    bool ok = __all_sync(0xffffffffu, bar_wait<PAIR>(bar(B_Q), 0u, abort_flag));
     uint32_t uk = 0, uv = 0;
     auto issue_qk = [&](uint32_t n) -> bool {
       const uint32_t units = n < n_cached ? cf::KU : 2 * cf::KU;
       const uint32_t d_tmem = tmem + T_S + (n & 1u) * 128u;
       for (uint32_t i = 0; i < units; ++i, ++uk) {
         const uint32_t st = uk % cf::NK;
-        if (!__all_sync(0xffffffffu, bar_wait(bar(B_K_FULL + st), (uk / cf::NK) & 1u, abort_flag))) return false;
+        if (!__all_sync(0xffffffffu, bar_wait<PAIR>(bar(B_K_FULL + st), (uk / cf::NK) & 1u, abort_flag))) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t qa = dq + (((i % cf::KU) * UNIT) >> 4), kb = dk + st * (UNIT >> 4);
+          const uint32_t qa = dq + (((i % cf::KU) * UNIT) >> 4), kb = dk + st * (cf::HAVE >> 4);
 #pragma unroll
           for (uint32_t j = 0; j < 16; ++j) {   // term, slab, 32 dims
-            const uint32_t o = ((j >> 2) & 1u) * (SLAB >> 4) + (j & 3u) * 2u;
-            mma_ss(d_tmem, desc(qa + (j >> 3) * ((BLK * D) >> 4) + o), desc(kb + o), IDESC, j == 0 ? i != 0u : 1u);
+            const uint32_t slab = (j >> 2) & 1u, kk = (j & 3u) * 2u;
+            const uint64_t a = desc(qa + (j >> 3) * ((BLK * D) >> 4) + slab * (SLAB >> 4) + kk), k = desc(kb + slab * (cf::HAVE >> 5) + kk);
+            if (PAIR) mma_ss_pair(d_tmem, a, k, IDESC, j == 0 ? i != 0u : 1u); else mma_ss(d_tmem, a, k, IDESC, j == 0 ? i != 0u : 1u);
           }
-          umma_commit(bar(B_K_EMPTY + st));
-          if (D != 256 && i + 1 == units) umma_commit(bar(B_S_FULL + (n & 1u)));
+          commit(B_K_EMPTY + st);
+          if (D != 256 && i + 1 == units) commit(B_S_FULL + (n & 1u));
         }
         __syncwarp();
       }
@@ -309,20 +369,27 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       const uint32_t keys = n < n_cached ? BLK : p.C - (n0 + n - ts.nA) * BLK;
       const uint32_t pt = tmem + T_S + (n & 1u) * 128u;
       for (uint32_t i = 0; i < units; ++i, ++uv) {
-        ok = __all_sync(0xffffffffu, i == 0 ? bar_wait(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag)
-                                            : bar_wait(bar(B_V2_FULL), (n - n_cached) & 1u, abort_flag));
+        ok = __all_sync(0xffffffffu, i == 0 ? bar_wait<PAIR>(bar(B_P_FULL + (n & 1u)), (n >> 1) & 1u, abort_flag)
+                                            : bar_wait<PAIR>(bar(B_V2_FULL), (n - n_cached) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t st = uv % cf::NV, vb = dv + st * (UNIT >> 4);
+          const uint32_t st = uv % cf::NV, vb = dv + st * (cf::HAVE >> 4);
 #pragma unroll
           for (uint32_t ks = 0; ks < 4; ++ks) {
             if (ks != 0 && ks * 32u >= keys) break;
-            mma_ts(tmem + T_O, pt + ks * 8u, desc(vb + ks * (4096u >> 4)), IDESC_P1, ks == 0 ? (n | i) != 0u : 1u);
-            mma_ts(tmem + T_O, pt + 32u + ks * 8u, desc(vb + ks * (4096u >> 4)), IDESC_P2, 1u);
+            const uint64_t v = desc(vb + ks * (4096u >> 4));
+            const uint32_t add = ks == 0 ? (n | i) != 0u : 1u;
+            if (PAIR) {
+              mma_ts_pair(tmem + T_O, pt + ks * 8u, v, IDESC_P1, add);
+              mma_ts_pair(tmem + T_O, pt + 32u + ks * 8u, v, IDESC_P2, 1u);
+            } else {
+              mma_ts(tmem + T_O, pt + ks * 8u, v, IDESC_P1, add);
+              mma_ts(tmem + T_O, pt + 32u + ks * 8u, v, IDESC_P2, 1u);
+            }
           }
-          umma_commit(bar(B_V_EMPTY + st));
-          if (n + 1 == n_local && i + 1 == units) umma_commit(bar(B_O));
+          commit(B_V_EMPTY + st);
+          if (n + 1 == n_local && i + 1 == units) commit(B_O);
         }
         __syncwarp();
       }
@@ -354,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
       valid_k[k] = Rk < rows_per_head;
       const uint32_t Rc = valid_k[k] ? Rk : 0u;
       row_k[k] = direct ? ((size_t(b) * p.C + Rc / p.G) * p.Hq + kvh * p.G + Rc % p.G) * D + z * 256u
-                        : (size_t(blockIdx.x) * BLK + rk) * 256u;
+                        : (size_t(slot) * BLK + rk) * 256u;
     }
 #pragma unroll 1
     for (uint32_t cc = 0; cc < 2; ++cc) {
@@ -388,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     const uint32_t R = mt * BLK + r;
     if (part == 0 && R < rows_per_head) {
       if (!direct)
-        p.ws_ml[size_t(blockIdx.x) * BLK + r] = make_float2(m_used, l);
+        p.ws_ml[size_t(slot) * BLK + r] = make_float2(m_used, l);
       else if (p.lse != nullptr && z == 0)
         p.lse[(size_t(b) * p.C + R / p.G) * p.Hq + kvh * p.G + R % p.G] =
             l == 0.f ? -INFINITY : (m_used - LIFT + log2f(l)) * 0.6931471805599453f;
@@ -403,8 +470,13 @@ __global__ void __launch_bounds__(THREADS, 1) dg_kv8_attn_kernel(const __grid_co
     }
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == W_MMA) tmem_dealloc(tmem, 512);
+  if (PAIR) {
+    cluster_sync_all();   // the leader's products read this CTA's memory, and its barriers take arrivals from here
+    if (warp == W_MMA) tmem_dealloc_pair(tmem, 512);
+  } else {
+    __syncthreads();
+    if (warp == W_MMA) tmem_dealloc(tmem, 512);
+  }
 }
 
 // Splits of a row joined: a row's 256 columns by WARPS warps, each a run of the splits in order, then the warps in order.  A
@@ -482,9 +554,14 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) dg_kv8_merge_ke
   if (p.lse != nullptr && z == 0 && w == 0 && lane == 0) p.lse[orow] = l == 0.f ? -INFINITY : (m - LIFT + log2f(l)) * 0.6931471805599453f;
 }
 
+template <uint32_t D, bool PAIR>
+static cudaError_t configure_one() {
+  return cudaFuncSetAttribute(dg_kv8_attn_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<D, PAIR>::SMEM));
+}
 cudaError_t configure_attn() {
-  cudaError_t e = cudaFuncSetAttribute(dg_kv8_attn_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<256>::SMEM));
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(dg_kv8_attn_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg<512>::SMEM));
+  cudaError_t e = configure_one<256, false>();
+  if (e == cudaSuccess) e = configure_one<512, false>();
+  if (e == cudaSuccess) e = configure_one<512, true>();
   return e;
 }
 
@@ -510,18 +587,26 @@ cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_
   return cudaLaunchKernelEx(&cfg, dg_kv8_merge_kernel<1>, p);
 }
 
-cudaError_t launch_attention(const AttnParams8& p, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st) {
+template <uint32_t D, bool PAIR>
+static cudaError_t launch_one(const AttnParams8& p, uint32_t n_ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_ctas);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = p.D == 256 ? Cfg<256>::SMEM : Cfg<512>::SMEM;
+  cfg.blockDim = dim3(Cfg<D, PAIR>::THREADS);
+  cfg.dynamicSmemBytes = Cfg<D, PAIR>::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = p.D == 256 ? cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<256>, p) : cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<512>, p);
+  cfg.numAttrs = PAIR ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, dg_kv8_attn_kernel<D, PAIR>, p);
+}
+cudaError_t launch_attention(const AttnParams8& p, bool pair, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st) {
+  const cudaError_t e = p.D == 256 ? launch_one<256, false>(p, n_ctas, st) : pair ? launch_one<512, true>(p, n_ctas, st) : launch_one<512, false>(p, n_ctas, st);
   return e != cudaSuccess || most_splits == 1 ? e : launch_merge(p, most_splits, st);
 }
 
