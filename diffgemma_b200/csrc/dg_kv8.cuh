@@ -371,7 +371,8 @@ cudaError_t launch_read(const ReadParams& p, cudaStream_t st);
 cudaError_t launch_token(const TokenParams& p, uint32_t D, uint32_t n_ctas, cudaStream_t st);
 cudaError_t launch_merge(const AttnParams8& p, uint32_t most_splits, cudaStream_t st);
 cudaError_t launch_attention(const AttnParams8& p, bool pair, uint32_t n_ctas, uint32_t most_splits, cudaStream_t st);
-cudaError_t launch_weights(const WeightParams& p, uint32_t D, uint32_t ctas, cudaStream_t st);
+// ctas: pairs of them where pair
+cudaError_t launch_weights(const WeightParams& p, uint32_t D, bool pair, uint32_t ctas, cudaStream_t st);
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t st);
 
 }  // namespace kv8

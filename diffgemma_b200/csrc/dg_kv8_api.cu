@@ -494,13 +494,16 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   // steps a CTA (1.3 us and less), 2 for what a run costs beside its steps, 4 for the launch.  us by runs / cut evenly, a canvas
   // of 256 over 2 KV heads of head_dim 256: 2,000 keys 30.7 / 22.1, 8,191 33.4 / 27.6, 19,200 59.2 / 43.0, 32,768 60.4 / 61.8,
   // 45,000 86.8 / 80.0; a canvas of 64, head_dim 512: 8,191 15.6 / 20.7, 19,200 36.7 / 30.8.
-  const uint32_t sms = c->num_sms > 0 ? uint32_t(c->num_sms) : 148u, kt = 512 / D, blocks = (n_keys + BLK - 1) / BLK;
+  const uint32_t rows = C * G, blocks = (n_keys + BLK - 1) / BLK;
+  const bool pair = D == 512 && rows >= 512;   // csrc/dg_kv8_weights.cu has both sides
+  const uint32_t sms = (c->num_sms > 0 ? uint32_t(c->num_sms) : 148u) / (pair ? 2u : 1u), kt = 512 / D * (pair ? 2u : 1u);
   {
     MaskParams mk = make_mask(*d, n_keys, 0, n_keys, 0);
     const uint32_t lo = mask_row_lo(mk, 0), last = (blocks + kt - 1) / kt - 1;
     p.run0 = lo / BLK / kt < last ? lo / BLK / kt : last;
   }
-  const uint32_t runs = ((blocks + kt - 1) / kt - p.run0) * p.Hkv, steps = (C * G * (D / 256) + BLK - 1) / BLK;
+  const uint32_t nr = D == 256 || pair ? 128u : 64u;   // rows of a step
+  const uint32_t runs = ((blocks + kt - 1) / kt - p.run0) * p.Hkv, steps = (rows + nr - 1) / nr;
   const uint64_t units = uint64_t(runs) * steps;
   uint32_t ctas = runs;
   const uint32_t whole = (runs + sms - 1) / sms * (steps + 2);
@@ -514,7 +517,7 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   }
   const uint64_t at = 0;
   DG_CUDA(kv8::launch_rows(qp, kv8::CodeParams{}, &at, 1, c->stream));
-  DG_CUDA(kv8::launch_weights(p, D, ctas, c->stream));
+  DG_CUDA(kv8::launch_weights(p, D, pair, ctas, c->stream));
   c->last_launches = p.part ? 3 : 2;
   return DG_OK;
 }

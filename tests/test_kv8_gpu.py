@@ -196,7 +196,8 @@ CASES = [
     (dict(n_q_heads=6, n_kv_heads=2), 100, 500, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 300, dict(mask_mode=CAUSAL)),
     (dict(n_q_heads=3, n_kv_heads=3), 7, 200, {}), (dict(n_q_heads=40, n_kv_heads=1), 33, 200, {}),
     ({**GLOBAL, "rotary_dim": 64}, 20, 300, {}), ({**GLOBAL, "rotary_dim": 0}, 20, 300, {}), ({**GLOBAL, "softmax_scale": 1.0}, 40, 900, {}),
-    (SLIDING, 8, 400, {}), (SLIDING, 9, 400, {}), (FULL, 2, 400, dict(mask_mode=CAUSAL)), (dict(n_q_heads=4, n_kv_heads=4), 8, 400, dict(mask_mode=CAUSAL)),
+    (SLIDING, 8, 400, {}), (SLIDING, 9, 400, {}), (FULL, 32, 1000, dict(mask_mode=CAUSAL)), (FULL, 256, 700, dict(window=90, mask_mode=PER_ROW)),
+    (FULL, 31, 500, dict(window=1, mask_mode=UNIFORM)), (FULL, 2, 400, dict(mask_mode=CAUSAL)), (dict(n_q_heads=4, n_kv_heads=4), 8, 400, dict(mask_mode=CAUSAL)),
     (dict(n_q_heads=4, n_kv_heads=4), 16, 400, {}), ({**FULL, "rotary_dim": 512, "rope_pairing": capi.ROPE_SPLIT_HALF}, 20, 300, {}),
 ]
 
@@ -374,7 +375,7 @@ def test_a_strong_first_token_loses_none_of_the_weak_ones(ctx, geo):
     (SLIDING, 256, 1500, dict(window=300, mask_mode=PER_ROW)), (SLIDING, 256, 1500, dict(window=300, mask_mode=UNIFORM)),
     (SLIDING, 200, 900, dict(window=100, mask_mode=CAUSAL)), (GLOBAL, 200, 900, dict(mask_mode=CAUSAL)), (FULL, 1, 300, {}), (FULL, 256, 700, {}),
     (FULL, 90, 400, dict(window=64, mask_mode=PER_ROW)), (SLIDING, 20, 9000, dict(window=300, mask_mode=PER_ROW)), (GLOBAL, 256, 9001, {}),
-    (FULL, 1, 5000, dict(window=2, mask_mode=CAUSAL)), (FULL, 256, 5000, {}), (dict(n_q_heads=6, n_kv_heads=2), 50, 300, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 9000, {})])
+    (FULL, 1, 5000, dict(window=2, mask_mode=CAUSAL)), (FULL, 256, 5000, {}), (FULL, 64, 4100, {}), (FULL, 65, 900, dict(window=200, mask_mode=CAUSAL)), (dict(n_q_heads=6, n_kv_heads=2), 50, 300, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 9000, {})])
 @pytest.mark.parametrize("decay", [0.0, 1.0, 0.25])
 def test_key_weights(ctx, geo, canvas, n, more, decay):
     layer = AttnLayer(canvas=canvas, **{**geo, **more})
