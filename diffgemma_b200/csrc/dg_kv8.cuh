@@ -86,7 +86,8 @@ __device__ __forceinline__ float sub_f32_f16(float x, uint16_t h) {
   asm("{\n\t.reg .b16 m;\n\tmov.b16 m, 0xBC00;\n\tfma.rn.f32.f16 %0, %1, m, %2;\n\t}" : "=f"(r) : "h"(h), "f"(x));
   return r;
 }
-// Four weights as e4m3 + e5m2: within 2^-8 of a weight down to 2^-6, within 2^-17 below
+// Four weights as e4m3 + e5m2: within 2^-8 of a weight down to 2^-6; below, within 2^-14 (the first term leaves at most 2^-10, the
+// second an eighth of half of that) and within 2^-3 of the weight
 __device__ __forceinline__ void split4(float a, float b, float c, float d, uint32_t* p1, uint32_t* p2) {
   *p1 = e4m3x4_half(a, b, c, d);
   const uint32_t lo = f16x2_from_e4m3x2(uint16_t(*p1)), hi = f16x2_from_e4m3x2(uint16_t(*p1 >> 16));

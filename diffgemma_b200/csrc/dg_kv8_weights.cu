@@ -19,28 +19,30 @@
 namespace dg {
 namespace kv8 {
 
+constexpr uint32_t W_EPI = 16, WW_LOAD = 16, WW_MMA = 17, W_THREADS = 18 * 32;
+// WB_Q_FULL of a stage counts its bytes and the sixteen warps that have read the scores of the stage before last: one wait for
+// the MMA warp.  WB_S_FULL says that the scores are there and the stage is free.
+// WB_C_EMPTY of each of the four places of row constants counts the warps that are done with them: they hold on to them longer than to
+// the scores, by any number of steps where a window's edge makes them look at every row.
+enum { WB_K = 0, WB_Q_FULL = 1, WB_S_FULL = 3, WB_C_EMPTY = 5, W_BARS = 9 };
+
 template <uint32_t D, bool PAIR> struct WCfg {
   static_assert(!PAIR || D == 512, "pairs: see above");
   static constexpr uint32_t KT = 512 / D, NR = D == 256 || PAIR ? 128 : 64;   // key tiles of a CTA, rows of a stage
   static constexpr uint32_t RUN = PAIR ? 2 * KT : KT, HR = PAIR ? NR / 2 : NR;   // key tiles of a run, rows of a stage in this CTA
   static constexpr uint32_t K_BYTES = KT * BLK * D, STAGE = 2 * HR * D;
   static constexpr uint32_t O_Q = K_BYTES, O_C = O_Q + 2 * STAGE, O_R = O_C + 4 * NR * 8, O_BAR = O_R + 4 * BLK * 4;
-  static constexpr uint32_t SMEM = O_BAR + 9 * 8 + 8;
+  static constexpr uint32_t SMEM = O_BAR + W_BARS * 8 + 8;
   static constexpr uint32_t COLS = KT * NR / 4;                          // score columns of an epilogue thread
   static constexpr uint32_t TM_COLS = 2 * KT * NR;
 };
-constexpr uint32_t W_EPI = 16, WW_LOAD = 16, WW_MMA = 17, W_THREADS = 18 * 32;
-// WB_Q_FULL of a stage counts its bytes and the sixteen warps that have read the scores of the stage before last: one wait for
-// the MMA warp.  WB_S_FULL says that the scores are there and the stage is free.
-enum { WB_K = 0, WB_Q_FULL = 1, WB_S_FULL = 3 };
-
 template <uint32_t D, bool PAIR>
 __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __grid_constant__ WeightParams p) {
   typedef WCfg<D, PAIR> cf;
   const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, cta = PAIR ? blockIdx.x >> 1 : blockIdx.x, ctas = PAIR ? gridDim.x >> 1 : gridDim.x;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s0 = smem_u32(smem);
-  volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + cf::O_BAR + 9 * 8);
+  volatile uint32_t* ctl = reinterpret_cast<volatile uint32_t*>(smem + cf::O_BAR + W_BARS * 8);
   volatile uint32_t* abort_flag = &ctl[0];
   auto bar = [&](uint32_t i) { return s0 + cf::O_BAR + i * 8u; };
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -58,6 +60,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
       mbar_init(bar(WB_Q_FULL + i), rank != 0u ? 1u : both * (W_EPI + 1u));
       mbar_init(bar(WB_S_FULL + i), 1u);
     }
+    for (uint32_t i = 0; i < 4; ++i) mbar_init(bar(WB_C_EMPTY + i), W_EPI);
     fence_mbar_init();
   }
   if (warp == WW_MMA) {
@@ -167,6 +170,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
               acc = add_f32x2(acc, pack_f32x2(x0, x1));
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(WB_C_EMPTY + (n & 3u)));
       }
       float a, b;
       unpack_f32x2(acc, a, b);
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
         for (uint32_t st = st0; st < st1; ++st, ++n) {
           const uint32_t sb = n & 1u, full = bar(WB_Q_FULL + sb);
           if (n > 1 && !bar_wait(bar(WB_S_FULL + sb), ((n - 2) >> 1) & 1u, abort_flag)) return false;
-          // the constants' slot was last read for step n - 4, which S^T of step n - 2 waited for
+          if (n > 3 && !bar_wait(bar(WB_C_EMPTY + (n & 3u)), ((n >> 2) - 1u) & 1u, abort_flag)) return false;
           mbar_expect_tx(full, cf::STAGE + cf::NR * 8u);
           const uint32_t dst = s0 + cf::O_Q + sb * cf::STAGE;
           const uint32_t R0 = st * cf::NR, mt = R0 / BLK;

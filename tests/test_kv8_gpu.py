@@ -375,7 +375,9 @@ def test_a_strong_first_token_loses_none_of_the_weak_ones(ctx, geo):
     (SLIDING, 256, 1500, dict(window=300, mask_mode=PER_ROW)), (SLIDING, 256, 1500, dict(window=300, mask_mode=UNIFORM)),
     (SLIDING, 200, 900, dict(window=100, mask_mode=CAUSAL)), (GLOBAL, 200, 900, dict(mask_mode=CAUSAL)), (FULL, 1, 300, {}), (FULL, 256, 700, {}),
     (FULL, 90, 400, dict(window=64, mask_mode=PER_ROW)), (SLIDING, 20, 9000, dict(window=300, mask_mode=PER_ROW)), (GLOBAL, 256, 9001, {}),
-    (FULL, 1, 5000, dict(window=2, mask_mode=CAUSAL)), (FULL, 256, 5000, {}), (FULL, 64, 4100, {}), (FULL, 65, 900, dict(window=200, mask_mode=CAUSAL)), (dict(n_q_heads=6, n_kv_heads=2), 50, 300, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 9000, {})])
+    (FULL, 1, 5000, dict(window=2, mask_mode=CAUSAL)), (FULL, 256, 5000, {}), (dict(n_q_heads=64, n_kv_heads=4), 33, 256, dict(window=5, mask_mode=UNIFORM)),
+    (dict(n_q_heads=12, n_kv_heads=4), 200, 4000, dict(window=64, mask_mode=CAUSAL)), (dict(n_q_heads=12, n_kv_heads=3), 129, 4000, dict(window=130, mask_mode=PER_ROW)),
+    ({**FULL, "n_q_heads": 32, "n_kv_heads": 2}, 100, 300, dict(window=40, mask_mode=UNIFORM)), (FULL, 64, 4100, {}), (FULL, 65, 900, dict(window=200, mask_mode=CAUSAL)), (dict(n_q_heads=6, n_kv_heads=2), 50, 300, {}), (dict(n_q_heads=5, n_kv_heads=1), 256, 9000, {})])
 @pytest.mark.parametrize("decay", [0.0, 1.0, 0.25])
 def test_key_weights(ctx, geo, canvas, n, more, decay):
     layer = AttnLayer(canvas=canvas, **{**geo, **more})
