@@ -140,7 +140,8 @@ def keep(weights, n, n_keep, n_recent):
 
 # A bf16 output of the kernels against these sums.  Rounding the output: half a bf16 step, 2^-8 of it.  A weight is the sum of
 # an e4m3 and an e5m2 number: 2^-4 of it left by the first, 2^-3 of that by the second, 2^-7, after a rounding to f16, 2^-11.
-# The largest exponent lag: weights below 2^-21 of the largest are held to 2^-22 of it.  Sums in fp32: 2^-24 of |p v| for each
+# Weights below 2^-11 of their row's largest are held to 2^-3 of themselves, 2^-19 of that largest at most: values to which no
+# larger weight adds anything can be that far off (the bound leaves it out, no case here has such values).  Sums in fp32: 2^-24 of |p v| for each
 # of T keys and two passes, far below.
 # Canvas values come as two codes: TAIL of the largest for those far below it.
 def out_bound(out, spread, T, canvas_top=0.0):

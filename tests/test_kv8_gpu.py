@@ -235,10 +235,10 @@ def test_many_splits(ctx, geo, canvas, splits):
     kv.close()
 
 
-@pytest.mark.parametrize("canvas", [1, 100])
-def test_two_contexts_at_once(ctx, canvas):
+@pytest.mark.parametrize("geo,canvas", [(GLOBAL, 1), (GLOBAL, 100), (FULL, 64)])
+def test_two_contexts_at_once(ctx, geo, canvas):
     """Two contexts, each with its own stream and scratch, over one cache at the same time."""
-    layer = AttnLayer(canvas=canvas, **GLOBAL)
+    layer = AttnLayer(canvas=canvas, **geo)
     kv, hk, hv = filled(ctx, layer, 9000, 4)
     ctx.synchronize()
     owns = [Context(0, make_current=False) for _ in range(2)]
@@ -416,7 +416,7 @@ def test_key_weights_add_up_to_the_rows(ctx):
 @pytest.mark.parametrize("geo,n,n_keep,n_recent", [
     (SLIDING, 1, 1, 0), (GLOBAL, 1, 1, 1), (GLOBAL, 300, 100, 0), (GLOBAL, 300, 300, 0), (GLOBAL, 300, 300, 300), (GLOBAL, 300, 17, 17),
     (SLIDING, 5003, 1250, 257), (FULL, 1000, 129, 1), (FULL, 2049, 2048, 3), (GLOBAL, 8193, 8192, 0), (GLOBAL, 20001, 5000, 1),
-    (GLOBAL, 150000, 4097, 100), (GLOBAL, 270000, 300, 7)])
+    (SLIDING, 40001, 1000, 5), (GLOBAL, 150000, 4097, 100), (GLOBAL, 270000, 300, 7)])
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
 def test_evict(ctx, geo, n, n_keep, n_recent, kind):
     layer = AttnLayer(**geo)
