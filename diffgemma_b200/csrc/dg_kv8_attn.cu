@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
       } else {
         there = bar_wait(bar(B_S_FULL + sb), (n >> 1) & 1u, abort_flag);
       }
-      if (!__all_sync(0xffffffffu, there)) break;
+      // (A wait that gave up ends nothing here: the warps of a row go through the same barriers to the end, and the status reports it.)
+      __all_sync(0xffffffffu, there);
       if (!warp_on) {
         // rows behind the last one: their P stays whatever it is, no row of the output reads it
         p_ready(sb);
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
       uint32_t s[32];
       tmem_ld32(t_lane + T_S + sb * 128u + part * 32u, s);
       // the maxima of the tile before have been read by all: their warps have arrived
-      if (n != 0 && !__all_sync(0xffffffffu, bar_wait(bar(B_P_FULL + (sb ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
+      if (n != 0) __all_sync(0xffffffffu, bar_wait(bar(B_P_FULL + (sb ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag));
       tmem_wait_ld();
       hide32(s, lo, hi, k0);
       k0 += BLK;
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
       const bool need = n == 0 || m_new > m_used + LAG;
       if (n != 0 && __any_sync(0xffffffffu, need)) {
         // the outputs of the tile before: its last V unit has been used
-        if (!wait_unit(B_V_EMPTY, cf::NV, n - 1u)) break;
+        wait_unit(B_V_EMPTY, cf::NV, n - 1u);
         tc_fence_after();
         const float alpha = need ? (m_used == -INFINITY ? 0.f : fast_exp2(m_used - m_new)) : 1.0f;
 #pragma unroll 1

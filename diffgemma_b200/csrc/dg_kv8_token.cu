@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
       const uint32_t sb = n & 1u;
       const int ek = ex.x, ev = ex.y;
       if (n + 1 < n_local) ex = *++ep;
-      if (!__all_sync(0xffffffffu, bar_wait(bar(TB_S + sb), (n >> 1) & 1u, abort_flag))) break;
+      // (A wait that gave up ends nothing here: a group's warps go through the same barriers to the end, and the status reports it.)
+      __all_sync(0xffffffffu, bar_wait(bar(TB_S + sb), (n >> 1) & 1u, abort_flag));
       tc_fence_after();
       uint32_t s1[8], s2[8];
       tmem_ld8(t_lane + TT_S + sb * NS + half * HR, s1);
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
           const float w = warp_max(x[j]);
           if (lane == 0) sm.red[warp][j] = w;
         }
-        if (n != 0 && !__all_sync(0xffffffffu, bar_wait(bar(TB_PV + (sb ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag))) break;
+        if (n != 0) __all_sync(0xffffffffu, bar_wait(bar(TB_PV + (sb ^ 1u)), ((n - 1u) >> 1) & 1u, abort_flag));
         tc_fence_after();
         bar_threads(bid, 128);
         float alpha[HR];
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
         bar_threads(bid, 128);                                      // the maxima have been read
       }
       // P of the tile before last has been used
-      if (n > 1 && !__all_sync(0xffffffffu, bar_wait(bar(TB_PV + sb), ((n - 2u) >> 1) & 1u, abort_flag))) break;
+      if (n > 1) __all_sync(0xffffffffu, bar_wait(bar(TB_PV + sb), ((n - 2u) >> 1) & 1u, abort_flag));
       const float back = pow2i(-ev);
       uint8_t* pt = smem + cf::O_P + sb * cf::P_BUF + (key & 15u);
 #pragma unroll

@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
       bool ok = true;
       for (uint32_t st = st0; st < st1; ++st, ++n) {
         const uint32_t sb = n & 1u;
-        ok = __all_sync(0xffffffffu, bar_wait(bar(WB_S_FULL + sb), (n >> 1) & 1u, abort_flag));
-        if (!ok) break;
+        // (a wait that gave up ends nothing here: all warps go through the same barriers, and nothing is stored)
+        if (!__all_sync(0xffffffffu, bar_wait(bar(WB_S_FULL + sb), (n >> 1) & 1u, abort_flag))) ok = false;
         tc_fence_after();
         const ulonglong2* cst = reinterpret_cast<const ulonglong2*>(smem + cf::O_C + (n & 3u) * cf::NR * 8u) + col0 / 2u;
         const uint32_t src = tmem + ((quarter * 32u) << 16) + sb * (cf::KT * cf::NR) + kt * cf::NR + col0;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) dg_kv8_weights_kernel(const __gr
         }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(W_EPI * 32) : "memory");
-      return ok;
+      return true;
     });
   } else if (warp == WW_LOAD) {
     if (lane == 0) {
