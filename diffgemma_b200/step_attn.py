@@ -62,7 +62,7 @@ def _addr(t):
     """A tensor's address as the C ABI takes it (None: NULL)."""
     if t is None:
         return None
-    assert t.is_contiguous(), "tensors handed to the C ABI must be contiguous"
+    assert t.is_cuda and t.is_contiguous(), "calls on 8-bit caches take contiguous tensors in device memory"
     return t.data_ptr()
 
 
@@ -278,7 +278,7 @@ class KvCache8:
         heads = self.layer.n_kv_heads
         if kept is None:
             kept = torch.empty((heads, n_keep), dtype=torch.int32, device=weights.device)
-        assert weights.dtype == torch.float32 and weights.shape[0] == heads and kept.shape == (heads, n_keep)
+        assert weights.dtype == torch.float32 and weights.shape[0] == heads and kept.dtype == torch.int32 and kept.shape == (heads, n_keep)
         assert weights_out is None or (weights_out.dtype == torch.float32 and weights_out.shape[0] == heads)
         st = self.ctx.lib.dg_kv8_evict(self.ctx.h, self.h, n_keys, _addr(weights), weights.shape[1], n_keep, n_recent, to.h, _addr(kept),
                                        _addr(weights_out), 0 if weights_out is None else weights_out.shape[1])
@@ -357,6 +357,8 @@ class CanvasAttention:
             assert k.shape == v.shape == (B, lay.canvas, lay.n_kv_heads, lay.head_dim) and k.dtype is v.dtype is torch.bfloat16
         if out is None:
             out = torch.empty_like(q)
+        else:
+            assert out.dtype is torch.bfloat16 and out.shape == q.shape
         lse = q.new_empty(rows, dtype=torch.float32) if with_lse else None
         q_rot = torch.empty_like(q) if with_q_rot else None
         handles, lens, places = self._arrays(B)
@@ -383,7 +385,8 @@ class CanvasAttention:
         """weights = decay * weights + what each cached key drew of the softmax of these rows (dg_kv8_key_weights).  q_rot
         [C,Hq,D] and lse [C,Hq] as denoise_kv8 returned them; weights: fp32 [Hkv, >= n_keys], updated in place."""
         lay = self.layer
-        assert q_rot.dtype == torch.bfloat16 and q_rot.shape[-3:] == (lay.canvas, lay.n_q_heads, lay.head_dim)
+        rows = lay.canvas * lay.n_q_heads
+        assert q_rot.dtype == torch.bfloat16 and q_rot.numel() == rows * lay.head_dim and lse.numel() == rows, "one canvas's rows"
         assert lse.dtype == weights.dtype == torch.float32 and weights.shape[0] == lay.n_kv_heads
         st = self.lib.dg_kv8_key_weights(self.ctx.h, self._desc_ref, kv.h, n_keys, _addr(q_rot), _addr(lse), _addr(weights),
                                          weights.shape[1], decay)

@@ -621,3 +621,26 @@ def test_refusals(ctx):
     ctx.synchronize()
     for c in (kv, other, to):
         c.close()
+
+
+def test_tensors_that_do_not_fit(ctx):
+    """What the C ABI cannot see (host memory, strides, types) is refused above it."""
+    layer = AttnLayer(canvas=4, **GLOBAL)
+    kv, _, _ = filled(ctx, layer, 100, 1, spare=28)
+    q, k, v, qw, kw = step_inputs(layer, 1, 5)
+    att = CanvasAttention(ctx, layer)
+    lse, w = torch.zeros(1, 4, 16, device=DEV), torch.zeros(2, 100, device=DEV)
+    for bad in (dict(q=q.cpu()), dict(q=q.float()), dict(q=q[:, :3]), dict(k=k.cpu()), dict(v=None), dict(out=torch.empty_like(q, dtype=torch.float32)),
+                dict(q=q.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises((AssertionError, AttributeError)):
+            att.denoise_kv8([kv], [100], **{**dict(q=q, k=k, v=v, qw=qw, kw=kw), **bad})
+    for bad in (dict(weights=w.cpu()), dict(weights=w.double()), dict(lse=lse[:, :3]), dict(q_rot=torch.cat([q, q]))):
+        with pytest.raises(AssertionError):
+            att.key_weights(kv, 100, **{**dict(q_rot=q, lse=lse, weights=w), **bad})
+    to = KvCache8(ctx, layer, 50)
+    for bad in (dict(weights=w.t().contiguous().t()), dict(kept=torch.empty(2, 50, dtype=torch.int64, device=DEV))):
+        with pytest.raises(AssertionError):
+            kv.evict_to(to, 100, **{**dict(weights=w, n_keep=50), **bad})
+    ctx.synchronize()
+    kv.close()
+    to.close()
