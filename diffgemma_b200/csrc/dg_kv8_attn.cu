@@ -192,17 +192,16 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
       const int ek = ex.x, ev = ex.y;
       ep = n + 1 == n_cached ? ec : ep + 1;
       if (n + 1 < n_local) ex = *ep;
-      // head_dim 256: the scores are there when the tile's last K unit (a canvas tile's second) has been used
+      // head_dim 256, a cached tile: the scores are there when its K unit has been used.  That unit's stage is used again by tile
+      // n + 2 at the earliest, whose scores wait for this warp's weights of tile n: the phase cannot pass unseen.  Two canvas tiles in a
+      // row are four units over three stages, so canvas tiles have barriers of their own, by turns: a second commit for each of them.
       bool there;
-      if (D == 256) {
+      if (D == 256 && n < n_cached) {
         there = bar_wait(bar(B_K_EMPTY) + stage * 8u, phase, abort_flag);
         if (++stage == cf::NK) { stage = 0; phase ^= 1u; }
-        if (n >= n_cached) {
-          there = there && bar_wait(bar(B_K_EMPTY) + stage * 8u, phase, abort_flag);
-          if (++stage == cf::NK) { stage = 0; phase ^= 1u; }
-        }
       } else {
-        there = bar_wait(bar(B_S_FULL + sb), (n >> 1) & 1u, abort_flag);
+        const uint32_t x = D == 256 ? n - n_cached : n;
+        there = bar_wait(bar(B_S_FULL + (x & 1u)), (x >> 1) & 1u, abort_flag);
       }
       // (A wait that gave up ends nothing here: the warps of a row go through the same barriers to the end, and the status reports it.)
       __all_sync(0xffffffffu, there);
@@ -327,7 +326,7 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
   } else if (warp == W_MMA && n_local > 0) {
     // The whole warp runs the loop, one elected lane issues.  A wait costs this warp some 150 cycles in which it issues nothing;
     // one before each group of 1,024 cycles of MMAs and one commit behind it keep the tensor pipe full (2,054 cycles for the 24
-    // MMAs of a 256-wide tile; two waits and two commits: 2,360), so V's bytes are counted where P's arrivals are and a K
+    // MMAs of a 256-wide tile; two waits and two commits: 2,360), so V's bytes are counted where P's arrivals are and a cached K
     // unit's release is the signal that scores are there.  Descriptors advance by adds on their low word (every operand lives
     // below 256 KB: the address field cannot carry).
     constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);           // 8-row groups 1024 apart, version 1, 128-byte swizzle
@@ -355,7 +354,7 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
             if (PAIR) mma_ss_pair(d_tmem, a, k, IDESC, j == 0 ? i != 0u : 1u); else mma_ss(d_tmem, a, k, IDESC, j == 0 ? i != 0u : 1u);
           }
           commit(B_K_EMPTY + st);
-          if (D != 256 && i + 1 == units) commit(B_S_FULL + (n & 1u));
+          if (i + 1 == units && (D != 256 || n >= n_cached)) commit(B_S_FULL + ((D == 256 ? n - n_cached : n) & 1u));
         }
         __syncwarp();
       }
