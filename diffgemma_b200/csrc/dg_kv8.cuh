@@ -9,10 +9,11 @@
 // token & 7 (the 128-byte swizzle of the UMMA descriptors), K as a K-major and V as an MN-major operand.  32 KB of a block
 // are one contiguous bulk copy; no tensor map is needed, so a launch over many caches carries two pointers for each.
 //
-// Scores and outputs as exact as the bf16 kernels': the operand that is not in the cache is split into two 8-bit terms,
-// q = q1 + q2 (e4m3 each, scaled by a power of two for each row; a bf16 number within 2^10 of its row's largest is exactly
-// such a sum) and p = p1 + p2 (e4m3 + e5m2).  kind::f8f6f4 runs at twice the bf16 rate, so two passes cost what one pass
-// over a bf16 cache costs, and no code is ever converted on its way to the tensor cores.
+// Scores and outputs as exact as the bf16 kernels': the operand that is not in the cache is split into 8-bit terms,
+// q = q1 + q2 (e4m3 each, scaled by a power of two for each row; a bf16 number within 2^9.8 of its row's largest is exactly
+// such a sum) and p = p1 + p2 + p3 (e5m2: 2^-11 of a weight down to 2^-18 of its row's largest).  kind::f8f6f4 runs at twice the bf16
+// rate, so a product takes one pass over a bf16 cache for Q and one and a half for P, and no code is ever converted on its way to the
+// tensor cores.
 #pragma once
 #include "dg_common.cuh"
 #include "sm100_ptx.cuh"
@@ -24,7 +25,8 @@ constexpr uint32_t BLK = 128;                  // tokens of a block
 constexpr uint32_t SLAB = BLK * 128;           // bytes of a slab: 128 tokens x 128 dims
 constexpr uint32_t UNIT = 2 * SLAB;            // what one bulk copy brings: 128 tokens x 256 dims
 constexpr int EXP_MIN = -60, EXP_MAX = 60;     // sums of scales of one row stay inside fp32
-constexpr float LIFT = 5.0f;                   // partial rows: weights stand at 2^LIFT times their reference
+constexpr float LIFT = 12.0f;                  // weights, and partial rows, stand at 2^LIFT times their reference
+constexpr uint32_t TERMS = 3;                  // e5m2 terms of a weight
 constexpr uint32_t MAX_SEQ = 64;               // caches served by one launch
 
 enum : uint32_t { KID_CODE = 16, KID_ATTN = 17, KID_WEIGHTS = 18, KID_EVICT = 19, KID_TOKEN = 20 };
@@ -55,26 +57,20 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t f16x2_from_e5m2x2(uint16_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(r) : "h"(v));
-  return r;
-}
+// bytes 0 and 1 (HIGH: 2 and 3) of four e5m2 numbers as f16: e5m2 is the upper byte of an f16.  A byte permutation, where the conversion
+// would wait for the unit that the exponentials need.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t f16x2_from_e5m2(uint32_t v) { return __byte_perm(v, 0u, HIGH ? 0x3424u : 0x1404u); }
 __device__ __forceinline__ uint32_t f16x2_from_e4m3x2(uint16_t v) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
   return r;
 }
 __device__ __forceinline__ float2 f32x2_from_e4m3x2(uint16_t v) { return unpack_f16x2(f16x2_from_e4m3x2(v)); }
-// Four fp32 (v[0] in the low byte) to e4m3 or e5m2 with the bits of `r` added below the last kept one: a half for each of the
-// four, which rounds to nearest (ties away from zero).  Two of the four take their bits mirrored.  One instruction for four
-// numbers, where conversions by pairs are two each and a byte permutation.
+// Four fp32 (a in the low byte) to e5m2 with the bits of `r` added below the last kept one: a half for each of the four, which
+// rounds to nearest (ties away from zero).  Two of the four take their bits mirrored.  One instruction for four numbers, where
+// conversions by pairs are two each and a byte permutation.
 constexpr uint32_t RS_HALF = 0x80018001u;
-__device__ __forceinline__ uint32_t e4m3x4_half(float a, float b, float c, float d) {
-  uint32_t r;
-  asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%4, %3, %2, %1}, %5;" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d), "r"(RS_HALF));
-  return r;
-}
 __device__ __forceinline__ uint32_t e5m2x4_half(float a, float b, float c, float d) {
   uint32_t r;
   asm("cvt.rs.satfinite.e5m2x4.f32 %0, {%4, %3, %2, %1}, %5;" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d), "r"(RS_HALF));
@@ -86,22 +82,15 @@ __device__ __forceinline__ float sub_f32_f16(float x, uint16_t h) {
   asm("{\n\t.reg .b16 m;\n\tmov.b16 m, 0xBC00;\n\tfma.rn.f32.f16 %0, %1, m, %2;\n\t}" : "=f"(r) : "h"(h), "f"(x));
   return r;
 }
-// Four weights as e4m3 + e5m2: within 2^-8 of a weight down to 2^-6; below, within 2^-14 (the first term leaves at most 2^-10, the
-// second an eighth of half of that) and within 2^-3 of the weight
-__device__ __forceinline__ void split4(float a, float b, float c, float d, uint32_t* p1, uint32_t* p2) {
-  *p1 = e4m3x4_half(a, b, c, d);
-  const uint32_t lo = f16x2_from_e4m3x2(uint16_t(*p1)), hi = f16x2_from_e4m3x2(uint16_t(*p1 >> 16));
-  *p2 = e5m2x4_half(sub_f32_f16(a, uint16_t(lo)), sub_f32_f16(b, uint16_t(lo >> 16)), sub_f32_f16(c, uint16_t(hi)), sub_f32_f16(d, uint16_t(hi >> 16)));
-}
-
-// Four weights as three e5m2 terms: within 2^-9 of a weight down to 2^-12, within 2^-17 below
-__device__ __forceinline__ void split4_e5m2(float a, float b, float c, float d, uint32_t (&t)[3]) {
+// Four weights as three e5m2 terms.  Three significant bits leave 2^-3 of a weight's power of two, a number of the format or less, so
+// that the next term starts four powers down: 2^-11 of a weight is left, and never less than 2^-17 (half the smallest step)
+__device__ __forceinline__ void split4_e5m2(float a, float b, float c, float d, uint32_t (&t)[TERMS]) {
   float x[4] = {a, b, c, d};
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (uint32_t i = 0; i < TERMS; ++i) {
     t[i] = e5m2x4_half(x[0], x[1], x[2], x[3]);
-    if (i == 2) break;
-    const uint32_t lo = f16x2_from_e5m2x2(uint16_t(t[i])), hi = f16x2_from_e5m2x2(uint16_t(t[i] >> 16));
+    if (i + 1 == TERMS) break;
+    const uint32_t lo = f16x2_from_e5m2<false>(t[i]), hi = f16x2_from_e5m2<true>(t[i]);
     x[0] = sub_f32_f16(x[0], uint16_t(lo));
     x[1] = sub_f32_f16(x[1], uint16_t(lo >> 16));
     x[2] = sub_f32_f16(x[2], uint16_t(hi));

@@ -246,11 +246,11 @@ kv8::QueryParams query_params(const dg_layer_desc& d, uint8_t* ws, const RowsLay
 }
 
 // How many splits the key tiles of each sequence are cut into, so that the launch's CTAs end together: `per` tiles a CTA at
-// most, all CTAs of a wave side by side.  Costs in key tiles of a CTA (1.45 us): ten for what a wave costs beside its tiles; the
+// most, all CTAs of a wave side by side.  Costs in key tiles of a CTA (1.6 us): ten for what a wave costs beside its tiles; the
 // merge, 2 us and the partial rows' way through memory, 0.33 ns for each row and split.  One canvas of 256 rows, us: 32,768 keys
-// of 2 KV heads, splits 1 / 2 / 3 / 4 / 5 / 7 / 9: 386 / 211 / 151 / 122 / 196 / 159 / 144; head_dim 512, 1 / 2 / 3 / 4 / 9: 468 / 289 /
-// 360 / 297 / 331; window 1024 of 8 KV heads, 1 / 2 / 3 / 4 / 5: 42 / 39 / 34 / 33 / 59; one token over 333 keys, 1 / 2 / 3: 18.8 /
-// 23.6 / 23.7.
+// of 2 KV heads, splits 1 / 2 / 3 / 4 / 5 / 7 / 9: 456 / 248 / 176 / 142 / 226 / 183 / 154; head_dim 512, 1 / 2 / 3 / 4 / 9: 560 / 324 /
+// 451 / 348 / 408; window 1024 of 8 KV heads, 1 / 2 / 3 / 4 / 5: 47 / 42 / 36 / 34 / 60; one token over 333 keys, 1 / 2 / 3: 11.8 /
+// 12.1 / 11.5.
 // Single tokens (dg_kv8_token_kernel) have all dims in one CTA and shorter tiles (1 us and less); the merge is a second launch of
 // 3 us behind 10.
 constexpr uint32_t kFixed8 = 10, kFixedToken = 6, kMerge8 = 1400, kMergeToken = 3500;

@@ -5,28 +5,31 @@
 // maximum and sum of the softmax:
 //   S = (q1 + q2) K          2 x D / 32 MMAs (M 128, N 128, K 32), K as the cache holds it
 //   x = s * c 2^ek + ev - m  the block's scales are powers of two: that of K multiplies, that of V shifts the exponent
-//   P = 2^x = p1 + p2        e4m3 + e5m2 in tensor memory, over the columns that S occupied
-//   O += (p1 + p2) V         8 MMAs (M 128, N 256, K 32)
+//   P = 2^x = p1 + p2 + p3   e5m2 each, in tensor memory, over the columns that S occupied
+//   O += (p1 + p2 + p3) V    12 MMAs (M 128, N 256, K 32)
 //   l += 2^-ev sum P         in fp32, from P before it is rounded
-// m follows the largest x with a lag of at most 2^LAG (O is rescaled only beyond it), so P <= 2^8 stays inside e4m3.  p2 in
-// e5m2 reaches 2^-16, 2^-21 of the largest weight: a strong first token beside 10^5 weak ones loses none of them.
+// m follows the largest x with a lag of at most 2^LAG (O is rescaled only beyond it), so P <= 2^15 stays inside e5m2.  Three terms hold
+// a weight to 2^-11 of itself down to 2^-18 of its row's largest, and to 2^-29 of that below: a strong first token without a
+// value beside 10^5 weak ones spoils none of them.
 // Tiles of the canvas come as two terms as well (K = k1 + k2, V = v1 + v2: the rows' bf16 values) and pass twice.
 //
-// Per 128 keys, 256 dims: 2,048 cycles of MMA, 64 KB from L2 / HBM, 16,384 exponentials (1,024 cycles), and 256 KB through
-// shared memory (S: 4 KB of Q and 4 KB of K for each MMA of 64 cycles; PV 64 KB; the copies 64 KB), which at 128 bytes a cycle
-// takes as long as the MMAs.  Measured: 2,600 cycles, the rest is the way from scores to weights and the waits between
-// (32,768 keys of 2 KV heads, 256 rows: 122 us).
-// head_dim 512: 3,072 cycles of MMA and 416 KB (3,328 cycles) a tile, 3,820 measured.  There two row tiles make a pair of CTAs
-// (cta_group::2, M = 256): each brings half of K's tokens and half of V's dims, so that copies and B operands halve (272 KB).
-// 256 rows over 2 KV heads, us alone / in pairs: 2,000 keys 47.6 / 46.7, 8,000 98.5 / 93.3, 32,000 313.6 / 285.9; a canvas
-// of 64, 32,000 keys 91.1 / 88.9.  head_dim 256 gains nothing (122 / 128: its tiles are too short to hide the other CTA's word).
+// Per 128 keys, 256 dims: 2,560 cycles of MMA, 64 KB from L2 / HBM, 16,384 exponentials (1,024 cycles), and 288 KB through
+// shared memory (S: 4 KB of Q and 4 KB of K for each MMA of 64 cycles; PV 96 KB; the copies 64 KB), which at 128 bytes a cycle
+// take 2,304.  Measured: 3,400 cycles, the rest is the way from scores to weights and the waits between (32,768 keys of 2 KV
+// heads, 256 rows: 148 us).  Two terms, e4m3 + e5m2, are 512 cycles of MMA less (123 us), but hold a weight at 2^-16 of its row's
+// largest to 2^-3 of itself only; a third term in the tiles that have such weights would be in nearly all of them.
+// head_dim 512: 3,584 cycles of MMA and 448 KB (3,584 cycles) a tile.  There two row tiles make a pair of CTAs
+// (cta_group::2, M = 256): each brings half of K's tokens and half of V's dims, so that copies and B operands halve (288 KB).
+// 256 rows over 2 KV heads, two terms, us alone / in pairs: 2,000 keys 47.6 / 46.7, 8,000 98.5 / 93.3, 32,000 313.6 / 285.9 (three
+// terms in pairs: 324); a canvas of 64, 32,000 keys 91.1 / 88.9.  head_dim 256 gains nothing (122 / 128: its tiles are too short to hide
+// the other CTA's word).
 #include "dg_kv8.cuh"
 
 namespace dg {
 namespace kv8 {
 
 constexpr uint32_t T_S = 0, T_O = 256;          // tensor memory: two S buffers of 128 columns, O
-constexpr float LAG = 3.0f;                     // 2^(LAG + LIFT) = 256 <= 448
+constexpr float LAG = 3.0f;                     // 2^(LAG + LIFT) = 32,768 <= 57,344
 constexpr uint32_t SM_WARPS = 16, W_K = 16, W_V = 17, W_MMA = 18, W_PASS = 19;   // W_PASS: CTA pairs only
 // B_P_FULL of a tile counts its softmax warps and the bytes of its first V unit; B_V2_FULL those of a canvas tile's second
 enum { B_Q = 0, B_O = 1, B_K_FULL = 2, B_K_EMPTY = 6, B_V2_FULL = 10, B_V_EMPTY = 11, B_S_FULL = 13, B_P_FULL = 15, B_V_OWN = 17, N_BARS = 19 };
@@ -47,8 +50,8 @@ template <uint32_t D, bool PAIR> struct Cfg {
 __device__ __forceinline__ void bar_sync_id(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-// 32 weights of a row from their scores: words of e4m3 codes and of e5m2 codes for every four; sums into ls
-__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t c2, uint64_t sh2, uint64_t (&ls)[2], uint32_t (&p1)[8], uint32_t (&p2)[8]) {
+// 32 weights of a row from their scores: a word of codes of each term for every four; sums into ls
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t c2, uint64_t sh2, uint64_t (&ls)[2], uint32_t (&p)[TERMS][8]) {
 #pragma unroll
   for (uint32_t e = 0; e < 32; e += 4) {
     float w[4];
@@ -59,7 +62,10 @@ __device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t c2, 
       w[2 * j + 1] = fast_exp2(w[2 * j + 1]);
       ls[j] = add_f32x2(ls[j], pack_f32x2(w[2 * j], w[2 * j + 1]));
     }
-    split4(w[0], w[1], w[2], w[3], &p1[e >> 2], &p2[e >> 2]);
+    uint32_t t[TERMS];
+    split4_e5m2(w[0], w[1], w[2], w[3], t);
+#pragma unroll
+    for (uint32_t i = 0; i < TERMS; ++i) p[i][e >> 2] = t[i];
   }
 }
 __device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
@@ -159,7 +165,7 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
   const uint32_t r = quarter * 32u + lane;
 
   if (warp < SM_WARPS) {
-    // What counts here is the time from a tile's scores to its weights: at most the 2,048 cycles of MMAs that are issued in
+    // What counts here is the time from a tile's scores to its weights: at most the 2,560 cycles of MMAs that are issued in
     // between.  So all sixteen warps work on one tile, four threads a row (two groups of eight on alternate tiles: 1,640 cycles
     // to the first half of P, 2,650 to the second).
     const uint32_t R = mt * BLK + r;
@@ -246,11 +252,11 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
       const float shift = (m_used == -INFINITY ? 0.f : -m_used) + float(ev) + LIFT;
       const uint64_t c2 = pack_f32x2(c, c), sh2 = pack_f32x2(shift, shift);
       uint64_t ls[2] = {0ull, 0ull};
-      uint32_t p1[8], p2[8];
-      weights32(s, c2, sh2, ls, p1, p2);
-      // the 32 keys of a thread are the K of one MMA: columns 8 part .. of p1, of p2 32 columns on
-      tmem_st8(t_lane + T_S + sb * 128u + part * 8u, p1);
-      tmem_st8(t_lane + T_S + sb * 128u + 32u + part * 8u, p2);
+      uint32_t pt[TERMS][8];
+      weights32(s, c2, sh2, ls, pt);
+      // the 32 keys of a thread are the K of one MMA: columns 8 part .. of p1, the other terms 32 columns on each
+#pragma unroll
+      for (uint32_t i = 0; i < TERMS; ++i) tmem_st8(t_lane + T_S + sb * 128u + i * 32u + part * 8u, pt[i]);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -325,14 +331,14 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
     }
   } else if (warp == W_MMA && n_local > 0) {
     // The whole warp runs the loop, one elected lane issues.  A wait costs this warp some 150 cycles in which it issues nothing;
-    // one before each group of 1,024 cycles of MMAs and one commit behind it keep the tensor pipe full (2,054 cycles for the 24
-    // MMAs of a 256-wide tile; two waits and two commits: 2,360), so V's bytes are counted where P's arrivals are and a cached K
+    // one before each group of 1,024 cycles of MMAs and one commit behind it keep the tensor pipe full (2,054 cycles for 24
+    // MMAs of a 256-wide tile, 8 of them PV; two waits and two commits: 2,360), so V's bytes are counted where P's arrivals are and a cached K
     // unit's release is the signal that scores are there.  Descriptors advance by adds on their low word (every operand lives
     // below 256 KB: the address field cannot carry).
     constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);           // 8-row groups 1024 apart, version 1, 128-byte swizzle
     auto desc = [](uint32_t lo) { return (uint64_t(HI) << 32) | uint64_t(lo); };
     constexpr uint32_t M = PAIR ? 256 : 128;
-    constexpr uint32_t IDESC = idesc_f8(M, 128, 0, 0), IDESC_P1 = idesc_f8(M, 256, 0, 1), IDESC_P2 = idesc_f8(M, 256, 1, 1);
+    constexpr uint32_t IDESC = idesc_f8(M, 128, 0, 0), IDESC_P = idesc_f8(M, 256, 1, 1);
     auto commit = [&](uint32_t b) { if (PAIR) commit_both(bar(b)); else umma_commit(bar(b)); };
     const uint32_t dq = ((s0 >> 4) & 0x3fffu) | (1u << 16), dk = (((s0 + cf::O_K) >> 4) & 0x3fffu) | (1u << 16);
     const uint32_t dv = (((s0 + cf::O_V) >> 4) & 0x3fffu) | ((SLAB >> 4) << 16);   // MN-major: 128-column chunks SLAB apart
@@ -380,12 +386,10 @@ __global__ void __launch_bounds__(Cfg<D, PAIR>::THREADS, 1) dg_kv8_attn_kernel(c
             if (ks != 0 && ks * 32u >= keys) break;
             const uint64_t v = desc(vb + ks * (4096u >> 4));
             const uint32_t add = ks == 0 ? (n | i) != 0u : 1u;
-            if (PAIR) {
-              mma_ts_pair(tmem + T_O, pt + ks * 8u, v, IDESC_P1, add);
-              mma_ts_pair(tmem + T_O, pt + 32u + ks * 8u, v, IDESC_P2, 1u);
-            } else {
-              mma_ts(tmem + T_O, pt + ks * 8u, v, IDESC_P1, add);
-              mma_ts(tmem + T_O, pt + 32u + ks * 8u, v, IDESC_P2, 1u);
+#pragma unroll
+            for (uint32_t t = 0; t < TERMS; ++t) {
+              const uint32_t a = pt + t * 32u + ks * 8u, on = t == 0 ? add : 1u;
+              if (PAIR) mma_ts_pair(tmem + T_O, a, v, IDESC_P, on); else mma_ts(tmem + T_O, a, v, IDESC_P, on);
             }
           }
           commit(B_V_EMPTY + st);

@@ -6,7 +6,7 @@
 //   S^T[key][row]  = K [q1 | q2]^T       D / 32 MMAs (M 128, N 32, K 32), the two halves added in fp32
 //   O^T[dim][row] += V^T [p1 | p2 | p3]^T  D / 32 MMAs (M 128, N 48, K 32), V^T as it lies (MN-major), P through shared memory
 // An MMA takes the 55 cycles that its 4 KB of the cache take, however few columns: 900 cycles, with the terms as columns of one
-// (as passes of N 16 each: 1,750).  So P has three terms, all e5m2 (one type a product): 2^-9, and a range of 2^33.
+// (as passes of N 16 each: 1,750).  So P has three terms, all e5m2 (one type a product), as in the kernel of whole canvases.
 // A thread of the softmax is a key and has the scores of half the rows in registers (two groups of four warps); a row's maximum is only looked for in the tiles
 // where some key exceeds what the exponents refer to by more than 2^LAG (one barrier says so), sums stay in the threads until
 // the end.  One CTA has all dims of a range of key tiles (head_dim 512 as well), five or six 32 KB units of K and V under way.
@@ -21,11 +21,11 @@ namespace kv8 {
 
 constexpr uint32_t NR = 16;                                         // query rows
 constexpr uint32_t PREP_WARPS = 12, TW_LOAD = 12, TW_MMA = 13, TT = 448;
-constexpr float TLAG = 3.0f, TLIFT = 12.0f;                         // 2^15 <= 57,344
+constexpr float TLAG = 3.0f;                                        // 2^(TLAG + LIFT) = 32,768 <= 57,344
 constexpr uint32_t HR = NR / 2;                                     // rows of a softmax thread
 // where row r stands among the columns: the even ones first, so that each group has half of however many there are
 __host__ __device__ __forceinline__ uint32_t slot_of(uint32_t r) { return (r & 1u) * HR + (r >> 1); }
-constexpr uint32_t TERMS = 3, NS = 2 * NR, NO = TERMS * NR;         // columns of a score and of an output accumulator
+constexpr uint32_t NS = 2 * NR, NO = TERMS * NR;         // columns of a score and of an output accumulator
 constexpr uint32_t TT_S = 0, TT_O = 2 * NS;                         // tensor memory: two S buffers, O of each 128 dims
 
 template <uint32_t D> struct TCfg {
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
         float top = -INFINITY, sum = 0.f;
         for (uint32_t c = 0; c < p.C; ++c) top = fmaxf(top, sc[c]);
         for (uint32_t c = 0; c < p.C; ++c) {
-          const float w = sc[c] == -INFINITY ? 0.f : fast_exp2(sc[c] - (top == -INFINITY ? 0.f : top) + TLIFT);   // (NaN stays)
+          const float w = sc[c] == -INFINITY ? 0.f : fast_exp2(sc[c] - (top == -INFINITY ? 0.f : top) + LIFT);   // (NaN stays)
           sum += w;
           sc[c] = w;
         }
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
         if (j >= nj) continue;
 #pragma unroll
         for (uint32_t i = j; i < j + 4; ++i) {
-          x[i] = fast_exp2(x[i] - (m[i] == -INFINITY ? 0.f : m[i]) + TLIFT);
+          x[i] = fast_exp2(x[i] - (m[i] == -INFINITY ? 0.f : m[i]) + LIFT);
           l[i] = fmaf(x[i], back, l[i]);
         }
         uint32_t w[TERMS];
@@ -415,9 +415,9 @@ __global__ void __launch_bounds__(TT, 1) dg_kv8_token_kernel(const __grid_consta
       if (j >= nj || key != j) continue;
       const uint32_t r = 2u * j + half;
       if (!direct) {
-        for (uint32_t z = 0; z < cf::KU; ++z) p.ws_ml[(size_t(blockIdx.x) * cf::KU + z) * BLK + r] = make_float2(m[j] - (TLIFT - LIFT), l[j]);
+        for (uint32_t z = 0; z < cf::KU; ++z) p.ws_ml[(size_t(blockIdx.x) * cf::KU + z) * BLK + r] = make_float2(m[j], l[j]);
       } else if (p.lse != nullptr) {
-        p.lse[(size_t(b) * p.C + r / p.G) * p.Hq + kvh * p.G + r % p.G] = l[j] == 0.f ? -INFINITY : (m[j] - TLIFT + log2f(l[j])) * 0.6931471805599453f;
+        p.lse[(size_t(b) * p.C + r / p.G) * p.Hq + kvh * p.G + r % p.G] = l[j] == 0.f ? -INFINITY : (m[j] - LIFT + log2f(l[j])) * 0.6931471805599453f;
       }
     }
   } else if (warp == TW_LOAD) {

@@ -1,9 +1,11 @@
 """Canvas rows over caches held in 8 bits: what the general tests of these calls leave out."""
+import math
+
 import pytest
 import torch
 
-from diffgemma_b200 import capi
-from diffgemma_b200.step_attn import AttnLayer, CanvasAttention, Context
+from diffgemma_b200.step_attn import AttnLayer, CanvasAttention, Context, KvCache8
+from tests import kv8_ref as ref
 from tests.test_kv8_gpu import FULL, GLOBAL, SLIDING, check_step, filled, step_inputs
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +37,38 @@ def test_two_canvas_tiles_in_one_cta(geo, canvas, n):
     kv.close()
     for own in owns:
         own.close()
+
+
+# A weight is held as three e5m2 numbers.  Rounding a number of [2^x, 2^(x + 1)) to three significant bits leaves 2^(x - 3) at most, which is
+# a number of the format itself, or less: the next term starts four powers of two down.  2^-3, 2^-7, 2^-11 of a weight are left; the smallest
+# step is 2^-16, so what is left may always be 2^-17 in the scale of the codes, where a row's largest weight stands at 2^12 to
+# 2^15.  A score is off by lse_bound at most; numerator and sum see it once each.
+def fine_bound(out, spread, big, D, T, v_top):
+    rel = 2.0 ** -11 + 2 * ref.lse_bound(big, D, T)[..., None] + (3 * T + 64) * 2.0 ** -24
+    return 2.0 ** -8 * out.abs() + rel * spread + T * 2.0 ** -29 * v_top
+
+
+@pytest.mark.parametrize("geo,canvas", [(GLOBAL, 1), (GLOBAL, 17), (GLOBAL, 40), (FULL, 2), (FULL, 9), (FULL, 32)])
+@pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("splits", [0, 1])
+def test_weak_weights_beside_a_strong_key_without_value(ctx, geo, canvas, n, splits):
+    """One key takes most of the weight and adds nothing (V = 0); all others draw the same, 2^-1 to 2^-20 of its weight.  Their errors do not
+    average out: the output is off by what one weight is."""
+    D = geo.get("head_dim", 256)
+    layer = AttnLayer(canvas=canvas, **{**geo, "rotary_dim": 0, "softmax_scale": 1.0, "v_norm": 0})
+    k, v = torch.zeros(n, 2, D, device=DEV), torch.ones(n, 2, D, device=DEV)
+    k[:, :, 0], k[0, :, 0], v[0] = 0.5, 1.0, 0.0
+    kv = KvCache8(ctx, layer, n)
+    kv.load(k.to(torch.bfloat16), v.to(torch.bfloat16), 0)
+    q = torch.zeros(1, canvas, 16, D, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    for bits in (1.3, 5.4, 9.2, 11.4, 13.3, 14.6, 15.7, 16.8, 18.55, 19.9):
+        qw = torch.full((D,), 2 * bits * math.log(2) / math.sqrt(D), device=DEV).to(torch.bfloat16)
+        ctx.set_splits(splits)
+        got = CanvasAttention(ctx, layer).denoise_kv8([kv], [n], q, None, None, qw, None)
+        ctx.set_splits(0)
+        qr, _, _ = ref.step_rows(layer, q[0], None, None, qw, None, n)
+        out, _, spread, big = ref.attend(layer, qr, ref.code(k.double()), ref.code(v.double()), ref.visible(layer, n, 0))
+        err = (got[0].double() - out).abs()
+        assert (err <= fine_bound(out, spread, big, D, n, 1.0)).all(), f"{bits}: off by {float((err / out).max()):.3g}"
+    kv.close()
