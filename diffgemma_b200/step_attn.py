@@ -66,6 +66,12 @@ def _addr(t):
     return t.data_ptr()
 
 
+def _norm_weight(w, layer):
+    """The weights of a row's norm: bf16, one for each dim (the C ABI sees an address only)."""
+    assert w is None or (w.dtype is torch.bfloat16 and w.numel() == layer.head_dim), "norm weights: bf16 [head_dim]"
+    return w
+
+
 class Context:
     """dg_ctx: one per host thread / stream."""
 
@@ -250,6 +256,7 @@ class KvCache8:
     def append(self, k: torch.Tensor, v: torch.Tensor, n_keys: int, pos: int | None = None, kw: torch.Tensor | None = None) -> None:
         """Raw k, v [n, Hkv, D] into slots [n_keys, n_keys + n): norm, RoPE at positions pos.. (None: n_keys), 8 bits."""
         n = self._rows(k, v)
+        kw = _norm_weight(kw, self.layer)
         st = self.ctx.lib.dg_kv8_append(self.ctx.h, self._desc_ref, self.h, n_keys, n_keys if pos is None else pos, n, _addr(k), _addr(v),
                                         _addr(kw))
         if st:
@@ -355,6 +362,7 @@ class CanvasAttention:
         assert q.dtype is torch.bfloat16 and q.shape == (*rows, lay.head_dim)
         if k is not None or v is not None:
             assert k.shape == v.shape == (B, lay.canvas, lay.n_kv_heads, lay.head_dim) and k.dtype is v.dtype is torch.bfloat16
+        qw, kw = _norm_weight(qw, lay), _norm_weight(kw, lay)
         if out is None:
             out = torch.empty_like(q)
         else:
