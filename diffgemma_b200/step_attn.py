@@ -58,11 +58,11 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr())
 
 
-def _addr(t):
+def _addr(t, device):
     """A tensor's address as the C ABI takes it (None: NULL)."""
     if t is None:
         return None
-    assert t.is_cuda and t.is_contiguous(), "calls on 8-bit caches take contiguous tensors in device memory"
+    assert t.is_cuda and t.get_device() == device and t.is_contiguous(), "calls on 8-bit caches take contiguous tensors in memory of the context's device"
     return t.data_ptr()
 
 
@@ -256,25 +256,25 @@ class KvCache8:
     def append(self, k: torch.Tensor, v: torch.Tensor, n_keys: int, pos: int | None = None, kw: torch.Tensor | None = None) -> None:
         """Raw k, v [n, Hkv, D] into slots [n_keys, n_keys + n): norm, RoPE at positions pos.. (None: n_keys), 8 bits."""
         n = self._rows(k, v)
-        kw = _norm_weight(kw, self.layer)
-        st = self.ctx.lib.dg_kv8_append(self.ctx.h, self._desc_ref, self.h, n_keys, n_keys if pos is None else pos, n, _addr(k), _addr(v),
-                                        _addr(kw))
+        kw, dev = _norm_weight(kw, self.layer), self.ctx.device
+        st = self.ctx.lib.dg_kv8_append(self.ctx.h, self._desc_ref, self.h, n_keys, n_keys if pos is None else pos, n, _addr(k, dev), _addr(v, dev),
+                                        _addr(kw, dev))
         if st:
             check(st, "dg_kv8_append")
 
     def load(self, k: torch.Tensor, v: torch.Tensor, n_keys: int = 0) -> None:
         """Rows that are ready (K normed and rotated already) into slots [n_keys, n_keys + n)."""
-        n = self._rows(k, v)
+        n, dev = self._rows(k, v), self.ctx.device
         if n:
-            check(self.ctx.lib.dg_kv8_load(self.h, n_keys, n, _addr(k), _addr(v)), "dg_kv8_load")
+            check(self.ctx.lib.dg_kv8_load(self.h, n_keys, n, _addr(k, dev), _addr(v, dev)), "dg_kv8_load")
 
     def read(self, slot0: int, n: int):
         """Slots [slot0, slot0 + n) as bf16 k, v [n, Hkv, D]."""
-        lay = self.layer
+        lay, dev = self.layer, self.ctx.device
         k = torch.empty((n, lay.n_kv_heads, lay.head_dim), dtype=torch.bfloat16, device=self._device)
         v = torch.empty_like(k)
         if n:
-            st = self.ctx.lib.dg_kv8_read(self.h, _addr(k), _addr(v), slot0, n)
+            st = self.ctx.lib.dg_kv8_read(self.h, _addr(k, dev), _addr(v, dev), slot0, n)
             if st:
                 check(st, "dg_kv8_read")
         return k, v
@@ -282,13 +282,13 @@ class KvCache8:
     def evict_to(self, to: "KvCache8", n_keys: int, weights: torch.Tensor, n_keep: int, n_recent: int = 0, kept=None, weights_out=None):
         """The n_recent last tokens and the n_keep - n_recent of largest weight before them, into `to` (dg_kv8_evict).
         weights: fp32 [Hkv, >= n_keys].  Returns the slots they had, int32 [Hkv, n_keep]."""
-        heads = self.layer.n_kv_heads
+        heads, dev = self.layer.n_kv_heads, self.ctx.device
         if kept is None:
             kept = torch.empty((heads, n_keep), dtype=torch.int32, device=weights.device)
         assert weights.dtype == torch.float32 and weights.shape[0] == heads and kept.dtype == torch.int32 and kept.shape == (heads, n_keep)
         assert weights_out is None or (weights_out.dtype == torch.float32 and weights_out.shape[0] == heads)
-        st = self.ctx.lib.dg_kv8_evict(self.ctx.h, self.h, n_keys, _addr(weights), weights.shape[1], n_keep, n_recent, to.h, _addr(kept),
-                                       _addr(weights_out), 0 if weights_out is None else weights_out.shape[1])
+        st = self.ctx.lib.dg_kv8_evict(self.ctx.h, self.h, n_keys, _addr(weights, dev), weights.shape[1], n_keep, n_recent, to.h, _addr(kept, dev),
+                                       _addr(weights_out, dev), 0 if weights_out is None else weights_out.shape[1])
         if st:
             check(st, "dg_kv8_evict")
         return kept
@@ -357,7 +357,7 @@ class CanvasAttention:
         """denoise() over caches held in 8 bits (dg_kv8_denoise).  q: [B,C,Hq,D], k, v: [B,C,Hkv,D] (None: the cached keys
         alone); n_keys and pos: cached tokens and first position of each canvas (pos None: n_keys).  Returns out, or a tuple
         with lse [B,C,Hq] and the rotated queries behind it where asked for."""
-        B, lay = len(kvs), self.layer
+        B, lay, dev = len(kvs), self.layer, self.ctx.device
         rows = (B, lay.canvas, lay.n_q_heads)
         assert q.dtype is torch.bfloat16 and q.shape == (*rows, lay.head_dim)
         if k is not None or v is not None:
@@ -374,8 +374,8 @@ class CanvasAttention:
         lens[:] = n_keys
         if pos is not None:
             places[:] = pos
-        st = self.lib.dg_kv8_denoise(self.ctx.h, self._desc_ref, handles, lens, None if pos is None else places, B, _addr(q), _addr(k),
-                                     _addr(v), _addr(qw), _addr(kw), _addr(out), _addr(lse), _addr(q_rot))
+        st = self.lib.dg_kv8_denoise(self.ctx.h, self._desc_ref, handles, lens, None if pos is None else places, B, _addr(q, dev), _addr(k, dev),
+                                     _addr(v, dev), _addr(qw, dev), _addr(kw, dev), _addr(out, dev), _addr(lse, dev), _addr(q_rot, dev))
         if st:
             check(st, "dg_kv8_denoise")
         if lse is None and q_rot is None:
@@ -392,11 +392,11 @@ class CanvasAttention:
     def key_weights(self, kv: KvCache8, n_keys: int, q_rot, lse, weights, decay: float = 1.0):
         """weights = decay * weights + what each cached key drew of the softmax of these rows (dg_kv8_key_weights).  q_rot
         [C,Hq,D] and lse [C,Hq] as denoise_kv8 returned them; weights: fp32 [Hkv, >= n_keys], updated in place."""
-        lay = self.layer
+        lay, dev = self.layer, self.ctx.device
         rows = lay.canvas * lay.n_q_heads
         assert q_rot.dtype == torch.bfloat16 and q_rot.numel() == rows * lay.head_dim and lse.numel() == rows, "one canvas's rows"
         assert lse.dtype == weights.dtype == torch.float32 and weights.shape[0] == lay.n_kv_heads
-        st = self.lib.dg_kv8_key_weights(self.ctx.h, self._desc_ref, kv.h, n_keys, _addr(q_rot), _addr(lse), _addr(weights),
+        st = self.lib.dg_kv8_key_weights(self.ctx.h, self._desc_ref, kv.h, n_keys, _addr(q_rot, dev), _addr(lse, dev), _addr(weights, dev),
                                          weights.shape[1], decay)
         if st:
             check(st, "dg_kv8_key_weights")

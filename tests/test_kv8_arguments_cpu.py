@@ -5,6 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from diffgemma_b200 import step_attn
 from diffgemma_b200.step_attn import AttnLayer, CanvasAttention, KvCache8
 
 
@@ -12,7 +13,10 @@ class NoCalls:
     """A library that no call may reach."""
 
     def __getattr__(self, name):
-        raise RuntimeError(f"{name} was called")
+        def call(*args):
+            raise RuntimeError(f"{name} was called")
+
+        return call
 
 
 LAYER = AttnLayer(canvas=4, n_kv_heads=2)
@@ -41,3 +45,31 @@ def test_norm_weights_of_an_append(bad):
     kv.ctx, kv.layer, kv.h, kv._desc_ref = CTX, LAYER, None, None
     with pytest.raises(AssertionError, match="norm weights"):
         kv.append(bf16(3, 2, 256), bf16(3, 2, 256), 0, kw=bad)
+
+
+def test_memory_of_another_device():
+    class OnDevice(SimpleNamespace):
+        is_cuda = True
+        get_device = lambda self: 1
+        is_contiguous = lambda self: True
+        data_ptr = lambda self: 64
+
+    assert step_attn._addr(OnDevice(), 1) == 64 and step_attn._addr(None, 1) is None
+    with pytest.raises(AssertionError, match="device"):
+        step_attn._addr(OnDevice(), 0)
+    with pytest.raises(AssertionError, match="device"):
+        step_attn._addr(bf16(1), 0)
+
+
+def test_every_address_is_checked_against_the_context():
+    """Host tensors stand for tensors of a device that is not the context's."""
+    att = CanvasAttention(CTX, LAYER)
+    kv = KvCache8.__new__(KvCache8)
+    kv.ctx, kv.layer, kv.h, kv._desc_ref = CTX, LAYER, None, None
+    rows = bf16(3, 2, 256)
+    w, lse = torch.zeros(2, 8), torch.zeros(4, 16)
+    kvs = [SimpleNamespace(h=C.c_void_p(1))]
+    for call in (lambda: att.denoise_kv8(kvs, [1], bf16(1, 4, 16, 256)), lambda: kv.append(rows, rows, 0), lambda: kv.load(rows, rows),
+                 lambda: att.key_weights(kv, 1, bf16(4, 16, 256), lse, w), lambda: kv.evict_to(kv, 4, w, 2)):
+        with pytest.raises(AssertionError, match="device"):
+            call()
