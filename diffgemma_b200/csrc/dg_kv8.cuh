@@ -201,6 +201,7 @@ struct QueryParams {
   const __nv_bfloat16* qw;     // [D] or null
   const float* lse;            // [C][Hq] or null
   __nv_bfloat16* q_rot;        // normed and rotated Q as bf16, or null
+  DevStatus* status;           // rows that are not finite are reported here (key weights)
   uint32_t prenormed;          // 1: q is normed and rotated already
   float eps, scale_log2;
   Rope rope;

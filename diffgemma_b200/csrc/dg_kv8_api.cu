@@ -471,6 +471,7 @@ extern "C" int32_t dg_kv8_key_weights(dg_ctx* c, const dg_layer_desc* d, dg_kv8*
   kv8::QueryParams qp = query_params(*d, c->kv8_rows, l, MT);
   qp.q = static_cast<const __nv_bfloat16*>(q_rot);
   qp.lse = lse;
+  qp.status = c->d_status;
   qp.prenormed = 1;
   qp.rope.half = 0;
   kv8::WeightParams p = {};

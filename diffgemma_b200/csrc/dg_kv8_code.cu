@@ -202,13 +202,30 @@ __global__ void __launch_bounds__(CT, NJ == 1 ? 2 : 1) dg_kv8_rows_kernel(const 
 #pragma unroll
       for (int j = 0; j < NJ; ++j) v[j] = make_uint4(0u, 0u, 0u, 0u);
     }
+    // key weights: the row's -log2 e * lse, -inf for a row that draws nothing
+    float nl = -INFINITY;
+    if (live && q.lse != nullptr) nl = -1.4426950408889634f * q.lse[(size_t(b) * o.C + i) * o.Hq + h];
     uint32_t top2 = 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) top2 = abs_max2(abs_max2(abs_max2(abs_max2(top2, v[j].x), v[j].y), v[j].z), v[j].w);
     uint32_t top = (top2 >> 16) > (top2 & 0xffffu) ? top2 >> 16 : top2 & 0xffffu;
     top = __reduce_max_sync(0xffffffffu, top);
     // a row that is not finite has no scores: its codes are NaN
-    const bool fin = top < 0x7f80u;
+    bool fin = top < 0x7f80u;
+    if (q.lse != nullptr) {
+      // no share of any key has a row without a sum (none, -lse = inf; or behind the last token), and one that is not finite or
+      // whose sum is not, which is reported: its NaN would be every key's, and a running mean's from then on
+      if (live && (!fin || !(nl < INFINITY && nl > -INFINITY))) {
+        if (lane == 0 && (!fin || nl != INFINITY)) dev_status_set(q.status, DG_DEV_NOT_FINITE, KID_CODE, blockIdx.x, i);
+        nl = -INFINITY;
+      }
+      if (nl == -INFINITY) {
+        top = 0u;
+        fin = true;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) v[j] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
     const int e = fin ? scale_exp(__uint_as_float(top << 16)) : 0;
     const float mul = fin ? pow2i(-e) : __uint_as_float(0x7fc00000u);
     uint8_t* dst = o.codes + ((size_t(b) * o.Hkv + kvh) * o.MT + R / BLK) * 2u * BLK * D;
@@ -221,12 +238,6 @@ __global__ void __launch_bounds__(CT, NJ == 1 ? 2 : 1) dg_kv8_rows_kernel(const 
       *reinterpret_cast<uint2*>(dst + BLK * D + off) = rest;
     }
     if (lane == 0) {
-      // -log2 e * lse; rows without a sum (none, or behind the last token) draw nothing
-      float nl = -INFINITY;
-      if (live && q.lse != nullptr) {
-        const float l = q.lse[(size_t(b) * o.C + i) * o.Hq + h];
-        nl = l == -INFINITY ? -INFINITY : -1.4426950408889634f * l;
-      }
       const size_t at = (size_t(b) * o.Hkv + kvh) * o.MT * BLK + R;
       if (q.lse != nullptr) {   // two rows' factors, then their -lse: as pairs
         float* pair = reinterpret_cast<float*>(o.row) + (at & ~size_t(1)) * 2u + (at & 1u);

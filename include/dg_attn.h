@@ -41,7 +41,8 @@ enum {
   DG_ERR_ALIGNMENT = -7,     /* a device pointer is not 16-byte aligned                         */
   DG_DEV_WAIT_TIMEOUT = 1,   /* a bounded device-side wait gave up (kernel unwound cleanly)     */
   DG_DEV_BAD_SHAPE = 2,      /* device-side shape assertion                                     */
-  DG_DEV_NOT_FINITE = 4,     /* a number that was to be held in 8 bits is not finite: it is held as zero */
+  DG_DEV_NOT_FINITE = 4,     /* a number that was to be held in 8 bits is not finite: it is held as zero (a row of
+                              * queries as rows of zeros that draw nothing)                      */
   DG_DEV_SMEM_LAYOUT = 3     /* a kernel's shared-memory map did not fit its (unaligned) window; it
                               * returned without doing anything                                  */
 };
@@ -355,7 +356,8 @@ int32_t dg_kv8_denoise(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* const* kv
 /* What each cached key drew of the softmax of one canvas's rows, added up over rows and the query heads of its KV head:
  *   weights[h * ld + t] = decay * weights[h * ld + t] + sum e^(score - lse),   t < n_keys
  * q_rot and lse as dg_kv8_denoise returned them for this canvas and cache; the mask is desc's (positions = slots).  decay 0:
- * weights is written without being read; 1: plain sums.                                                                 */
+ * weights is written without being read; 1: plain sums.  A row with lse = -inf draws nothing; nor does one whose query or lse is
+ * not finite otherwise, and DG_DEV_NOT_FINITE is reported.                                                              */
 int32_t dg_kv8_key_weights(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* kv, uint32_t n_keys, const void* q_rot, const float* lse,
                            float* weights, uint64_t ld, float decay);
 /* Keeps n_keep of n_keys tokens of each KV head in `to`, in order: the last n_recent, and of those before them the

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from diffgemma_b200 import capi
 from diffgemma_b200.step_attn import AttnLayer, CanvasAttention, Context, KvCache8
 from tests import kv8_ref as ref
 from tests.test_kv8_gpu import FULL, GLOBAL, SLIDING, check_step, filled, step_inputs
@@ -71,4 +72,40 @@ def test_weak_weights_beside_a_strong_key_without_value(ctx, geo, canvas, n, spl
         out, _, spread, big = ref.attend(layer, qr, ref.code(k.double()), ref.code(v.double()), ref.visible(layer, n, 0))
         err = (got[0].double() - out).abs()
         assert (err <= fine_bound(out, spread, big, D, n, 1.0)).all(), f"{bits}: off by {float((err / out).max()):.3g}"
+    kv.close()
+
+
+# ------------------------------------------------------------------------------------------------- rows that are not numbers
+@pytest.mark.parametrize("geo,canvas,n", [(GLOBAL, 1, 300), (GLOBAL, 40, 2000), (FULL, 9, 700), (FULL, 64, 3000), (SLIDING, 256, 1500)])
+@pytest.mark.parametrize("decay", [0.0, 0.5])
+def test_rows_that_are_not_finite_draw_nothing(ctx, geo, canvas, n, decay):
+    """A query that is not finite has no softmax, and so no share of a key: the weights of all others stay what they are, and the
+    status says what was left out.  The same for a log-sum-exp that is not a number beside a good query."""
+    layer = AttnLayer(canvas=canvas, **geo)
+    kv, hk, _ = filled(ctx, layer, n, 7)
+    q, k, v, qw, kw = step_inputs(layer, 1, 3)
+    q[0, 0, 1, 5], q[0, canvas - 1, 9, 0] = math.inf, math.nan
+    att = CanvasAttention(ctx, layer)
+    _, lse, q_rot = att.denoise_kv8([kv], [n], q, k, v, qw, kw, with_lse=True, with_q_rot=True)
+    bad = torch.zeros(canvas, 16, dtype=torch.bool, device=DEV)
+    bad[0, 1] = bad[canvas - 1, 9] = True
+    assert torch.equal(torch.isnan(lse[0]), bad) and torch.equal(torch.isnan(q_rot[0]).any(-1), bad)
+    assert ctx.device_status()[0] == 0
+    lse[0, canvas // 2, 3], lse[0, canvas // 2, 12], lse[0, 0, 14] = math.nan, math.inf, -math.inf
+    w0 = torch.rand(layer.n_kv_heads, n, device=DEV)
+    w = att.key_weights(kv, n, q_rot[0], lse[0], w0.clone(), decay=decay)
+    assert ctx.device_status()[:2] == (capi.DG_DEV_NOT_FINITE, 16)
+    ctx.lib.dg_ctx_clear_device_status(ctx.h)
+    out = ~torch.isfinite(lse[0])
+    assert int(out.sum()) == 5
+    gone = lse[0].masked_fill(out, -math.inf)
+    qr = q_rot[0].double().masked_fill(out[..., None], 0.0)
+    see = ref.visible(layer, n, 0)
+    want = ref.key_weights(layer, qr, hk, see, gone) + decay * w0.double()
+    _, _, _, big = ref.attend(layer, qr, hk, hk, see)
+    rel = float(ref.lse_bound(big.flatten(1).amax(1), layer.head_dim, canvas * 16 // layer.n_kv_heads))
+    assert ((w.double() - want).abs() <= rel * want + 1e-37).all()
+    # without a row that is not finite nothing is reported, and the same weights come out
+    again = att.key_weights(kv, n, qr.to(torch.bfloat16), gone, w0.clone(), decay=decay)
+    assert torch.equal(again, w) and ctx.device_status()[0] == 0
     kv.close()
