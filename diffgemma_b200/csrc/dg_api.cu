@@ -26,6 +26,11 @@
 
 using namespace dg;
 
+std::string& dg::host::last_error() {
+  static thread_local std::string text;
+  return text;
+}
+
 // ------------------------------------------------------------------------------------------
 // objects
 // ------------------------------------------------------------------------------------------
@@ -93,7 +98,7 @@ static int32_t make_kv_tmap(CUtensorMap* tm, void* base, uint64_t cap, uint32_t 
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
-    g_last_error = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(int(r));
+    last_error() = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(int(r));
     return DG_ERR_CUDA;
   }
   return DG_OK;
@@ -188,7 +193,7 @@ static int32_t ensure_bits(dg_ctx* ctx, size_t tiles) {
 // ------------------------------------------------------------------------------------------
 // context
 // ------------------------------------------------------------------------------------------
-extern "C" const char* dg_last_error_message(void) { return g_last_error.c_str(); }
+extern "C" const char* dg_last_error_message(void) { return last_error().c_str(); }
 
 extern "C" const char* dg_status_str(int32_t s) {
   switch (s) {
@@ -1560,7 +1565,7 @@ NcclApi& nccl() {
   return api;
 }
 int32_t fail_nccl(ncclResult_t r, const char* what) {
-  g_last_error = std::string(what) + ": " + (nccl().GetErrorString ? nccl().GetErrorString(r) : "nccl error");
+  last_error() = std::string(what) + ": " + (nccl().GetErrorString ? nccl().GetErrorString(r) : "nccl error");
   return DG_ERR_NCCL;
 }
 }  // namespace
@@ -1720,7 +1725,7 @@ extern "C" int32_t dg_attention_static_scratch(dg_ctx* c, const dg_layer_desc* d
                            (d->head_dim == 512 ? 2u : 1u);
   const uint32_t row_limit = kStaticRows;
   if (rows > row_limit || q_tiles > kStaticTiles) {
-    g_last_error = "dg_attention_static_scratch: canvas * n_q_heads = " + std::to_string(rows) + " rows (" +
+    last_error() = "dg_attention_static_scratch: canvas * n_q_heads = " + std::to_string(rows) + " rows (" +
                    std::to_string(q_tiles) + " query tiles) exceeds the built-in scratch of " +
                    std::to_string(row_limit) + " rows / " + std::to_string(kStaticTiles) +
                    " tiles; use dg_attention, which allocates its workspace";

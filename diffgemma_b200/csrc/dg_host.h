@@ -12,13 +12,22 @@
 
 using namespace dg;
 
+// Not for other objects of the process: no name here leaves the library (an inline variable would otherwise be one for the whole
+// process, whichever library defined it).
+namespace dg {
+namespace host __attribute__((visibility("hidden"))) {}
+}  // namespace dg
+using namespace dg::host;
+
 // ------------------------------------------------------------------------------------------
 // error plumbing
 // ------------------------------------------------------------------------------------------
-inline thread_local std::string g_last_error;
+namespace dg {
+namespace host {
+std::string& last_error();           // this thread's (dg_api.cu)
 
 inline int32_t fail_cuda(cudaError_t e, const char* what) {
-  g_last_error = std::string(what) + ": " + cudaGetErrorString(e);
+  last_error() = std::string(what) + ": " + cudaGetErrorString(e);
   return DG_ERR_CUDA;
 }
 #define DG_CUDA(call)                                \
@@ -28,9 +37,11 @@ inline int32_t fail_cuda(cudaError_t e, const char* what) {
   } while (0)
 
 inline int32_t fail(int32_t code, const char* msg) {
-  g_last_error = msg;
+  last_error() = msg;
   return code;
 }
+}  // namespace host
+}  // namespace dg
 
 // ------------------------------------------------------------------------------------------
 // the context
@@ -96,6 +107,8 @@ struct dg_ctx {
 // ------------------------------------------------------------------------------------------
 // checks, scratch
 // ------------------------------------------------------------------------------------------
+namespace dg {
+namespace host {
 inline int32_t check_desc(const dg_layer_desc* d) {
   if (!d) return fail(DG_ERR_INVALID_ARG, "desc is NULL");
   if (d->n_q_heads == 0 || d->n_kv_heads == 0 || d->n_q_heads % d->n_kv_heads != 0)
@@ -148,3 +161,5 @@ inline int32_t grow_scratch(dg_ctx* ctx, A** a, size_t na, B** b, size_t nb, siz
   cudaThreadExchangeStreamCaptureMode(&mode);
   return e == cudaSuccess ? DG_OK : fail_cuda(e, "scratch allocation");
 }
+}  // namespace host
+}  // namespace dg
