@@ -7,7 +7,7 @@ import torch
 from diffgemma_b200 import capi
 from diffgemma_b200.step_attn import AttnLayer, CanvasAttention, Context, KvCache8
 from tests import kv8_ref as ref
-from tests.test_kv8_gpu import FULL, GLOBAL, SLIDING, check_step, filled, step_inputs
+from tests.test_kv8_gpu import CASES, FULL, GLOBAL, SLIDING, check_step, filled, step_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -109,3 +109,91 @@ def test_rows_that_are_not_finite_draw_nothing(ctx, geo, canvas, n, decay):
     again = att.key_weights(kv, n, qr.to(torch.bfloat16), gone, w0.clone(), decay=decay)
     assert torch.equal(again, w) and ctx.device_status()[0] == 0
     kv.close()
+
+
+@pytest.mark.parametrize("geo,canvas,n", [(GLOBAL, 1, 700), (FULL, 2, 900), (GLOBAL, 30, 2000), (FULL, 15, 2000), (FULL, 64, 3000), (SLIDING, 256, 900)])
+@pytest.mark.parametrize("splits", [0, 1, 3, 7, 20])
+def test_a_query_that_is_not_finite_spoils_its_row_alone(ctx, geo, canvas, n, splits):
+    """On every form of the kernel, whole and through both merges: the other rows keep their bits."""
+    layer = AttnLayer(canvas=canvas, **geo)
+    kv, _, _ = filled(ctx, layer, n, 7)
+    q, k, v, qw, kw = step_inputs(layer, 1, 3)
+    att = CanvasAttention(ctx, layer)
+    ctx.set_splits(splits)
+    good, lse_good = att.denoise_kv8([kv], [n], q, k, v, qw, kw, with_lse=True)
+    rows = [(0, 1), (canvas - 1, 15), (canvas // 2, 8)]
+    for (i, h), x in zip(rows, (math.inf, math.nan, -math.inf)):
+        q[0, i, h, 17 * h] = x
+    out, lse = att.denoise_kv8([kv], [n], q, k, v, qw, kw, with_lse=True)
+    ctx.set_splits(0)
+    bad = torch.zeros(canvas, 16, dtype=torch.bool, device=DEV)
+    for i, h in rows:
+        bad[i, h] = True
+    assert torch.isnan(out[0][bad]).all() and torch.isnan(lse[0][bad]).all()
+    assert torch.equal(out[0][~bad], good[0][~bad]) and torch.equal(lse[0][~bad], lse_good[0][~bad])
+    assert ctx.device_status()[0] == 0
+    kv.close()
+
+
+# ------------------------------------------------------------------------------------------------- bounds, batches
+@pytest.mark.parametrize("geo,canvas,n,more", CASES)
+def test_outputs_within_what_three_terms_hold(ctx, geo, canvas, n, more):
+    layer = AttnLayer(canvas=canvas, **{**geo, **more})
+    kv, hk, hv = filled(ctx, layer, n, 100 + n)
+    q, k, v, qw, kw = step_inputs(layer, 1, n + 1)
+    got = CanvasAttention(ctx, layer).denoise_kv8([kv], [n], q, k, v, qw, kw)
+    qr, kr, vr = ref.step_rows(layer, q[0], k[0], v[0], qw, kw, n)
+    keys, values = torch.cat([hk[:n], kr]), torch.cat([hv[:n], vr])
+    out, _, spread, big = ref.attend(layer, qr, keys, values, ref.visible(layer, n, canvas))
+    T = keys.shape[0]
+    # a canvas value is two codes, TAIL of the largest off where it is far below it
+    bound = fine_bound(out, spread, big, layer.head_dim, T, float(values.abs().max())) + 1.01 * ref.TAIL * float(vr.abs().max())
+    err = (got[0].double() - out).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    kv.close()
+
+
+@pytest.mark.parametrize("canvas", [15, 20, 64])
+def test_batches_of_unequal_lengths_at_head_dim_512(ctx, canvas):
+    """Canvases of one and of several row tiles (alone and in pairs of CTAs) over caches of unequal lengths, one of them twice."""
+    layer = AttnLayer(canvas=canvas, **FULL)
+    lens = [0, 1, 700, 128, 129, 3000]
+    held = [filled(ctx, layer, n, 10 * i) for i, n in enumerate(lens)]
+    held.append(held[2])
+    lens.append(300)
+    q, k, v, qw, kw = step_inputs(layer, len(held), 77)
+    pos = [n + 3 * i for i, n in enumerate(lens)]
+    out, lse = CanvasAttention(ctx, layer).denoise_kv8([h[0] for h in held], lens, q, k, v, qw, kw, pos=pos, with_lse=True)
+    for b, n in enumerate(lens):
+        check_step(layer, out[b], lse[b], q[b], k[b], v[b], qw, kw, n, pos[b], *held[b][1:])
+    for h in held[:-1]:
+        h[0].close()
+
+
+@pytest.mark.parametrize("geo,canvas", [(GLOBAL, 2), (GLOBAL, 60), (FULL, 2), (FULL, 15), (FULL, 64)])
+def test_what_two_terms_would_leave_is_not_there(ctx, geo, canvas):
+    """Two groups of keys whose values are opposite and whose weights nearly cancel, a little differently in every row: the output is small
+    and its rounding with it, so that the weights' own errors show."""
+    D = geo.get("head_dim", 256)
+    layer = AttnLayer(canvas=canvas, **{**geo, "rotary_dim": 0, "softmax_scale": 1.0, "v_norm": 0})
+    n = 256
+    k, v, q, qw = opposite_groups(n, canvas, D)
+    kv = KvCache8(ctx, layer, n)
+    kv.load(k.to(DEV), v.to(DEV), 0)
+    q, qw = q.to(DEV), qw.to(DEV)
+    got = CanvasAttention(ctx, layer).denoise_kv8([kv], [n], q, None, None, qw, None)
+    qr, _, _ = ref.step_rows(layer, q[0], None, None, qw, None, n)
+    out, _, spread, big = ref.attend(layer, qr, ref.code(k.double().to(DEV)), ref.code(v.double().to(DEV)), ref.visible(layer, n, 0))
+    err = (got[0].double() - out).abs()
+    assert (err <= fine_bound(out, spread, big, D, n, 1.0)).all()
+    kv.close()
+
+
+def opposite_groups(n, canvas, D):
+    """Keys along two dims with values 1 and -1, queries a few hundredths of a radian off the diagonal."""
+    k, v = torch.zeros(n, 2, D, dtype=torch.bfloat16), torch.ones(n, 2, D, dtype=torch.bfloat16)
+    k[0::2, :, 0], k[1::2, :, 1], v[1::2] = 1.0, 1.0, -1.0
+    turn = math.pi / 4 + 0.1 * (torch.rand(canvas, 16, generator=torch.Generator().manual_seed(5), dtype=torch.float64) - 0.5)
+    q = torch.zeros(1, canvas, 16, D, dtype=torch.bfloat16)
+    q[0, :, :, 0], q[0, :, :, 1] = turn.cos(), turn.sin()
+    return k, v, q, torch.full((D,), 3.0 / math.sqrt(D)).to(torch.bfloat16)
