@@ -2,8 +2,8 @@
 //
 // Rows that a step rounds to bf16 (queries, canvas K and V) are normed and rotated in 64 bits: a score is a sum over one
 // row's elements, and an element that a 32-bit intermediate puts on the other side of a rounding border moves every score
-// of its row.  Appended rows, which end in 3 mantissa bits, take 32.  Angles are in 64 bits everywhere: at position 131,072
-// a 32-bit angle is off by up to 0.008.
+// of its row.  Appended rows, which end in 3 mantissa bits, take 32.  Angles are 64-bit, since a 32-bit one is off by up to 0.008 at
+// position 131,072; an append looks up the first token's of each run of up to 16 and turns on from there in 32 bits (2^-20 at most).
 #pragma once
 #include "dg_kv8.cuh"
 

@@ -263,7 +263,8 @@ class KvCache8:
             check(st, "dg_kv8_append")
 
     def load(self, k: torch.Tensor, v: torch.Tensor, n_keys: int = 0) -> None:
-        """Rows that are ready (K normed and rotated already) into slots [n_keys, n_keys + n)."""
+        """Rows that are ready (K normed and rotated already) into slots [n_keys, n_keys + n).  Keys of a KvCache bring its 32-bit
+        angles along (up to 0.008 rad off at position 131,072); append() of the raw rows does not."""
         n, dev = self._rows(k, v), self.ctx.device
         if n:
             check(self.ctx.lib.dg_kv8_load(self.h, n_keys, n, _addr(k, dev), _addr(v, dev)), "dg_kv8_load")

@@ -323,13 +323,13 @@ int32_t dg_attn_denoise_topk(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv* kv, 
  *
  * K and V of each KV head are e4m3 codes with one power-of-two scale for each block of 128 slots:
  *   value = code * 2^e,  e = the smallest integer in [-60, 60] with (largest magnitude of the block) <= 448 * 2^e,
- * codes rounded to nearest even.  A value carries four significant bits down to 2^-14 of its block's largest and an absolute
- * error of 2^-19 of that below it.  What is not finite cannot be held: it is stored as zero and DG_DEV_NOT_FINITE is
+ * codes rounded to nearest even.  A value carries four significant bits down to 2^(e - 6), which is 2^-13.8 of its block's largest or
+ * less, and below it an absolute error of 2^(e - 10), 2^-17.8 of that largest at most.  What is not finite cannot be held: it is stored as zero and DG_DEV_NOT_FINITE is
  * reported.  head_dim 256 or 512, rotary_dim a multiple of 16; linear caches.
  *
  * Tokens sit in slots [0, n_keys); the caller keeps n_keys.  RoPE positions are given apart from slots, because after an
- * eviction they differ: `pos` is the position of the first new token.  Angles are computed in 64 bits (dg_kv_append's are
- * 32-bit: up to 0.008 apart at position 131,072).  All pointers are device pointers unless said otherwise.              */
+ * eviction they differ: `pos` is the position of the first new token.  A step's angles are 64-bit,
+ * an appended key's within 2^-20 of those (dg_kv_append's are 32-bit: up to 0.008 apart at position 131,072).  All pointers are device pointers unless said otherwise.              */
 typedef struct dg_kv8 dg_kv8;
 int32_t dg_kv8_create(dg_ctx* ctx, const dg_layer_desc* desc, uint64_t capacity_tokens, dg_kv8** out);
 int32_t dg_kv8_destroy(dg_kv8* kv);
@@ -339,7 +339,9 @@ uint64_t dg_kv8_capacity(const dg_kv8* kv);      /* capacity_tokens rounded up t
  * that holds tokens already is coded again as a whole, from the values it holds, at the scale that old and new need.     */
 int32_t dg_kv8_append(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* kv, uint64_t n_keys, uint64_t pos, uint64_t n,
                       const void* k, const void* v, const void* kw);
-/* The same for rows that are ready (K normed and rotated already), on the stream of the cache's context.                */
+/* The same for rows that are ready (K normed and rotated already), on the stream of the cache's context.  Keys read from a bf16
+ * cache (dg_kv_read) bring that cache's 32-bit angles along, while dg_kv8_denoise rotates its queries by 64-bit ones: far out,
+ * where those 0.008 matter, dg_kv8_append of the raw rows is the better way.                                            */
 int32_t dg_kv8_load(dg_kv8* kv, uint64_t n_keys, uint64_t n, const void* k, const void* v);
 /* Slots [slot0, slot0 + n) as bf16 [n][Hkv][D] (exact), ordered on the context's stream; does not synchronise.          */
 int32_t dg_kv8_read(dg_kv8* kv, void* k_out, void* v_out, uint64_t slot0, uint64_t n);
@@ -349,7 +351,9 @@ int32_t dg_kv8_read(dg_kv8* kv, void* k_out, void* v_out, uint64_t slot0, uint64
  * zeros.  pos[b] (host array; NULL: n_keys) is the position of canvas row 0.  A window counts positions and needs
  * pos[b] = n_keys[b].  The same cache may serve several canvases.  out: bf16 [batch][C][Hq][D]; lse (or NULL): fp32
  * [batch][C][Hq], ln of the sum of e^score over what a row sees, -inf where it sees nothing; q_rot (or NULL): the normed
- * and rotated queries, bf16 [batch][C][Hq][D].  Outputs overlap neither inputs nor each other.                          */
+ * and rotated queries, bf16 [batch][C][Hq][D].  Outputs overlap neither inputs nor each other.  A softmax weight is held to 2^-11
+ * of itself down to 2^-18 of its row's largest, and to 2^-29 of that below.  A query that is not finite gives NaN in its own row
+ * of out and lse.                                                                                                       */
 int32_t dg_kv8_denoise(dg_ctx* ctx, const dg_layer_desc* desc, dg_kv8* const* kv, const uint32_t* n_keys, const uint64_t* pos,
                        uint32_t batch, const void* q, const void* k, const void* v, const void* qw, const void* kw, void* out,
                        float* lse, void* q_rot);
